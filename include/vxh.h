@@ -479,6 +479,93 @@ int vxh_attention_rows(const float *q, int M, int n_past, int n_ctx, int n_heads
 size_t vxh_attention_rows_workspace_floats(int M, int n_ctx, int cap, int n_heads, int n_kv_heads,
                                            int head_dim);
 
+/* ---- paged KV cache in 8 bits ---------------------------------------------------
+ * A pool of pages of 32, 64 or 128 tokens that several requests share, a
+ * request's pages listed in its row of a page table, the keys and values in
+ * 8 bits with one fp32 scale per page and kv head.  No counterpart in the
+ * reference, which keeps one fp32 cache per model (src/model.c:404-411).
+ *
+ * A step of serving is
+ *   vxh_page_tables     lengths -> pages, row starts, row positions, slots
+ *   vxh_kvq_write       the step's (rotated) k and v rows into their slots
+ *   vxh_attention_kvq   the step's q rows over their requests' tokens
+ * with no host synchronisation: every length, table and slot is read on the
+ * device, so a captured graph of a step can be replayed with others.  A slot
+ * is page * page_size + offset; -1 (or one past the pool) names none.
+ *
+ * Value of a code = code * scale: VXH_KVQ_INT8 holds whole numbers -127..127,
+ * VXH_KVQ_E4M3 the OCP fp8 format (largest value 448).
+ * Layout, per page and kv head (page * n_kv_heads + head, page * head_dim
+ * bytes): [token / 32][dim / 32][lane 64][16 bytes], lane = 16 g + n.
+ *   k  bytes 0-7: dims 8g..8g+7 of token n, bytes 8-15: of token n + 16
+ *   v  bytes 0-7: dim n of tokens 4g..4g+3, 16+4g..16+4g+3; bytes 8-15: dim n+16
+ * (of the 32 tokens and 32 dims); an int8 byte is code + 128. */
+enum { VXH_KVQ_INT8 = 1, VXH_KVQ_E4M3 = 2 };
+typedef struct {
+    int type;          /* VXH_KVQ_INT8 or VXH_KVQ_E4M3                         */
+    int page;          /* tokens per page: 32, 64 or 128                       */
+    int n_pages;
+    int n_kv_heads;
+    int head_dim;      /* 32, 64, 96 or 128                                    */
+    void *k, *v;       /* device, codes                                        */
+    float *ks, *vs;    /* device, [n_pages][n_kv_heads]                        */
+} vxh_kvq;
+/* n_pages * page slots, at most 2^31 - 1; the cache starts as zeros. */
+int vxh_kvq_alloc(vxh_kvq *c, int type, int page, int n_pages, int n_kv_heads, int head_dim);
+int vxh_kvq_free(vxh_kvq *c);
+
+#define VXH_PAGE_MAX_SEQS 4096
+#define VXH_PAGE_MAX_ROWS (1 << 18)
+#define VXH_KVQ_MAX_ROWS 8192
+/* Pages, rows and slots of one step, from the lengths: request b < n_seqs has
+ * len[b] tokens cached and adds add[b] rows (negative: none).  Its new pages
+ * are the next of free_pages[n_free], in order of requests:
+ *   table[b * ld_table + j]   entries of the new pages; others stay
+ *   len_out[b] = len[b] + add[b]         (may not lie over len or add)
+ *   row0[b], b <= n_seqs      rows before request b
+ *   row_pos[r], slot[r], r < max_rows    position and slot of row r, -1 behind
+ *                             the last row
+ *   counts[0..3] = rows, pages taken from the front of free_pages, 0, pages needed
+ * A step that does not fit changes no table entry: len_out = len, every row0
+ * is 0 and every slot -1 (so that the step's other calls do nothing), and
+ * counts[2] is a sum of 1 (too few free pages), 2 (more than max_rows rows)
+ * and 4 (a request past ld_table pages). */
+int vxh_page_tables(const int *len, const int *add, int n_seqs, int page, const int *free_pages, int n_free,
+                    int *table, int ld_table, int *len_out, int *row0, int *row_pos, int *slot, int max_rows,
+                    int *counts, vxh_stream s);
+/* k[R][ldk], v[R][ldv] (fp32, [kv head][dim] each, 16-byte aligned, ld % 4 ==
+ * 0) into slot[r]; R <= VXH_KVQ_MAX_ROWS.  Per page and head, with A the
+ * largest finite magnitude the call writes there and top = 127 or 448:
+ *   scale = A / top (0 where A < 2^-100) if the call writes the page's first
+ *           token, which starts the page anew, else max(its scale, A / top)
+ *   code  = nearest(x / scale), ties to even; infinities +-top, NaN 0
+ * and where the scale grew, the tokens already on the page are rounded again
+ * at the new one.  Two rows of one slot: the later row stays.  Rows whose slot
+ * names no page are left out. */
+int vxh_kvq_write(const vxh_kvq *c, const float *k, int ldk, const float *v, int ldv, const int *slot, int R,
+                  vxh_stream s);
+/* The inverse: k[r], v[r] = code * scale of slot[r]; rows of no slot stay as
+ * they are. */
+int vxh_kvq_read(const vxh_kvq *c, const int *slot, int R, float *k, int ldk, float *v, int ldv, vxh_stream s);
+/* Causal attention of a ragged batch: rows row0[b]..row0[b+1]-1 of q[max_rows]
+ * [ldq] are the last tokens of request b, which has len[b] tokens in the cache
+ * (as vxh_page_tables leaves them in row0 and len_out); row i of m sits at
+ * position len[b] - m + i and reads positions [0, min(position + 1, cap)) (cap
+ * 0: all) of the pages table[b * ld_table ..].  Head h uses kv head h *
+ * n_kv_heads / n_heads.  A row that reads nothing is zeros; rows behind the
+ * last request stay as they were.  What the cache holds past the positions a
+ * request's rows read may be anything; a table entry that is no page counts as
+ * positions nobody reads, and lengths past ld_table pages end there.
+ * max_seq_rows is the largest number of rows a request is expected to have;
+ * only speed depends on it.  q and out 16-byte aligned, ldq and ld_out
+ * multiples of 4.  The partial results of requests cut into segments live in
+ * ws->part (vxh_attention_kvq_workspace_floats): one workspace serves one
+ * stream at a time. */
+int vxh_attention_kvq(const float *q, int ldq, const int *row0, const int *len, int n_seqs, int max_rows,
+                      int max_seq_rows, const int *table, int ld_table, int n_heads, const vxh_kvq *c, int cap,
+                      float *out, int ld_out, vxh_workspace *ws, vxh_stream s);
+size_t vxh_attention_kvq_workspace_floats(int max_rows, int n_seqs, int n_heads, int n_kv_heads, int head_dim);
+
 /* ---- elementwise ------------------------------------------------------------- */
 /* y[m][i] += x[m][i] for i < n (residual add, src/model.c:546, :589). */
 int vxh_add_rows(float *y, int ldy, const float *x, int ldx, int M, int n, vxh_stream s);
