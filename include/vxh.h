@@ -267,7 +267,8 @@ typedef struct {
 } vxh_epilogue;
 
 /* Per-stream scratch: the fp64 GEMM accumulator of vxh_gemm (allocated
- * zeroed, left zeroed by every call) and the attention partials. */
+ * zeroed, left zeroed by every call; completion counters of
+ * vxh_attention_kvq lie behind it) and the attention partials. */
 typedef struct {
     double *acc;
     size_t acc_elems;
@@ -559,8 +560,9 @@ int vxh_kvq_read(const vxh_kvq *c, const int *slot, int R, float *k, int ldk, fl
  * max_seq_rows is the largest number of rows a request is expected to have;
  * only speed depends on it.  q and out 16-byte aligned, ldq and ld_out
  * multiples of 4.  The partial results of requests cut into segments live in
- * ws->part (vxh_attention_kvq_workspace_floats): one workspace serves one
- * stream at a time. */
+ * ws->part (vxh_attention_kvq_workspace_floats) of a workspace that
+ * vxh_workspace_alloc made (it holds the call's counters too): one workspace
+ * serves one stream at a time. */
 int vxh_attention_kvq(const float *q, int ldq, const int *row0, const int *len, int n_seqs, int max_rows,
                       int max_seq_rows, const int *table, int ld_table, int n_heads, const vxh_kvq *c, int cap,
                       float *out, int ld_out, vxh_workspace *ws, vxh_stream s);

@@ -1,56 +1,651 @@
 // Attention of a ragged batch over the paged 8-bit KV cache.
+//
+// A request's rows and the G = n_heads / n_kv_heads query heads of one kv head
+// make up its queries there (query i: row i / G, head i % G), taken in tiles.
+// The work is the list of all (request, kv head, tile, 32-token group); every
+// workgroup takes an equal, consecutive piece of it, so lengths may differ as
+// they like: a long request spreads over many workgroups, short ones share
+// one.  A tile cut by a piece's ends leaves partial results (maximum, sum,
+// weighted values) in the workspace, joined in order by the last workgroup
+// that contributes to it.
 #include "vxh_kvq.h"
 
-// One wavefront per (row, head): lane l keeps a running maximum, sum and
-// output over tokens l, l + 64, ..; the lanes join at the end.
-template <int TYPE, int HD>
-__global__ __launch_bounds__(64) void vx_attention_kvq_kernel(const float *__restrict__ q, int ldq,
-                                                              const int *__restrict__ row0, const int *__restrict__ len,
-                                                              int B, int max_rows, const int *__restrict__ table,
-                                                              int ld_table, int n_heads, vxh_kvq c, int cap,
-                                                              float *__restrict__ out, int ld_out)
+typedef float vx_f32x4 __attribute__((ext_vector_type(4)));
+
+#define AK_WAVES 4
+#define AK_THREADS (64 * AK_WAVES)
+#define AK_WG 512                // pieces: two workgroups per CU
+#define AK_BEGIN 8               // what beginning and ending a tile costs, in 32-token groups
+#define AK_SMALL 8               // tiles of up to this many groups take a wavefront each
+#define AK_JOIN 8                // parts whose loads are in flight together
+#define AK_BLOCK 16              // parts one workgroup joins
+#define AK_SNAP 12
+
+// ---------------------------------------------------------------------------
+// The work list.  Every workgroup counts it anew from the lengths (they are on
+// the device only): a thread sums a run of requests, the runs are scanned.
+// ---------------------------------------------------------------------------
+struct vx_kvq_batch {
+    const int *row0, *len;
+    int B, max_rows, n_kv, G, cap, limit;    // limit: tokens a table row can name
+};
+
+struct vx_kvq_seq {
+    int row, m, n, end, nq;      // first row, rows, tokens, tokens any row reads, queries per kv head
+};
+
+__device__ __forceinline__ vx_kvq_seq vx_kvq_request(const vx_kvq_batch &a, int b)
 {
-    const int r = blockIdx.x, h = blockIdx.y, kvh = h / (n_heads / c.n_kv_heads), lane = threadIdx.x;
-    int b = -1;
-    for (int i = 0; i < B; i++)
-        if (row0[i] <= r && r < row0[i + 1]) b = i;
-    if (b < 0) return;
-    const int n = min(len[b], (int)min((int64_t)ld_table * c.page, (int64_t)0x7FFFFFFF));
-    int end = n - (row0[b + 1] - r) + 1;
-    if (cap > 0) end = min(end, cap);
-    const float *qr = q + (size_t)r * ldq + h * HD;
-    float m = -INFINITY, l = 0.0f, o[HD];
-#pragma unroll
-    for (int d = 0; d < HD; d++) o[d] = 0.0f;
-    for (int t = lane; t < end; t += 64) {
-        const int page = table[(size_t)b * ld_table + t / c.page];
-        if ((unsigned)page >= (unsigned)c.n_pages) continue;
-        const size_t hp = (size_t)page * c.n_kv_heads + kvh, base = hp * (size_t)(c.page * HD);
-        const uint8_t *kp = (const uint8_t *)c.k + base, *vp = (const uint8_t *)c.v + base;
-        float s = 0.0f;
-#pragma unroll 8
-        for (int d = 0; d < HD; d++) s = fmaf(qr[d], vx_kvq_value<TYPE>(kp[vx_kvq_k_byte(t % c.page, d, HD)]), s);
-        s *= c.ks[hp] / sqrtf((float)HD);
-        const float nm = fmaxf(m, s), f = expf(m - nm), p = expf(s - nm);
-        m = nm;
-        l = l * f + p;
-#pragma unroll
-        for (int d = 0; d < HD; d++)
-            o[d] = o[d] * f + p * (vx_kvq_value<TYPE>(vp[vx_kvq_v_byte(t % c.page, d, HD)]) * c.vs[hp]);
+    vx_kvq_seq s;
+    s.row = min(max(a.row0[b], 0), a.max_rows);
+    s.m = max(min(a.row0[b + 1], a.max_rows) - s.row, 0);
+    s.n = min(max(a.len[b], 0), a.limit);
+    s.end = a.cap > 0 ? min(s.n, a.cap) : s.n;
+    s.nq = s.m * a.G;
+    return s;
+}
+
+// 32-token groups of every tile of one kv head (at least one: a tile that
+// reads nothing still writes its zeros).
+__device__ __forceinline__ int vx_kvq_groups(const vx_kvq_seq &s) { return max((s.end + 31) >> 5, 1); }
+
+// Items of a tile: its groups, behind AK_BEGIN that stand for what beginning
+// and ending a tile cost.
+__device__ __forceinline__ int vx_kvq_weight(const vx_kvq_seq &s) { return vx_kvq_groups(s) + AK_BEGIN; }
+
+// 8 codes to fp16, exactly.
+template <int TYPE>
+__device__ __forceinline__ vx_half8 vx_kvq_half8(uint32_t a, uint32_t b)
+{
+    vx_half2 h[4];
+    if (TYPE == VXH_KVQ_INT8) {
+        // 0x64xx is 1024 + xx
+        const vx_half2 off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+        h[0] = __builtin_bit_cast(vx_half2, __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u)) + off;
+        h[1] = __builtin_bit_cast(vx_half2, __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u)) + off;
+        h[2] = __builtin_bit_cast(vx_half2, __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u)) + off;
+        h[3] = __builtin_bit_cast(vx_half2, __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)) + off;
+    } else {
+        h[0] = __builtin_bit_cast(vx_half2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, false));
+        h[1] = __builtin_bit_cast(vx_half2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, true));
+        h[2] = __builtin_bit_cast(vx_half2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, false));
+        h[3] = __builtin_bit_cast(vx_half2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, true));
     }
-    const float all = vx_wave_max64(m), f = m > -INFINITY ? expf(m - all) : 0.0f;
-    l = vx_wave_sum64(l * f);
+    return vx_half8{h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
+}
+
+// x = hi + lo to 22 bits (both truncated, so the two add up with one sign).
+__device__ __forceinline__ void vx_split(float a, float b, vx_half2 *hi, vx_half2 *lo)
+{
+    *hi = __builtin_bit_cast(vx_half2, __builtin_amdgcn_cvt_pkrtz(a, b));
+    *lo = __builtin_bit_cast(vx_half2, __builtin_amdgcn_cvt_pkrtz(a - (float)(*hi)[0], b - (float)(*hi)[1]));
+}
+
+// MFMA sources stay live past the instruction: a destination in VGPRs that
+// overlaps them gives wrong values.
+#define AK_KEEP(D, A, B) asm("" : "+v"(D) : "v"(A), "v"(B))
+
+__device__ __forceinline__ void vx_dev_store2(float *p, float a, float b)
+{
+    __hip_atomic_store((uint64_t *)p, __builtin_bit_cast(uint64_t, make_float2(a, b)), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 vx_dev_load2(const float *p)
+{
+    return __builtin_bit_cast(float2,
+                              __hip_atomic_load((const uint64_t *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
+// Quotient of two counts; 64-bit division only where they need it.
+__device__ __forceinline__ int64_t vx_quot(int64_t a, int64_t b)
+{
+    return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
+__device__ __forceinline__ int64_t vx_uniform(int64_t v)
+{
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+    return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
+// A place in the list: a tile of a request and kv head, and its first item.
+struct vx_kvq_found {
+    vx_kvq_seq s;
+    int b, nth;                  // request; tile of the request, over its kv heads
+    int64_t first;
+};
+
+struct vx_kvq_list {
+    int64_t at[AK_THREADS + 1];      // items before each thread's run of requests
+    vx_kvq_seq one[AK_THREADS];      // a run's last request (its only one up to AK_THREADS requests)
+    int64_t wave[AK_WAVES];
+    int tiles[AK_WAVES];
+    vx_kvq_found found[2];
+};
+
+__device__ __forceinline__ void vx_kvq_run(const vx_kvq_batch &a, int *b0, int *b1)
+{
+    const int E = (a.B + AK_THREADS - 1) / AK_THREADS;
+    *b0 = min((int)threadIdx.x * E, a.B);
+    *b1 = min(*b0 + E, a.B);
+}
+
+// Items of the whole list.
+template <int QT>
+__device__ __forceinline__ int64_t vx_kvq_scan(const vx_kvq_batch &a, vx_kvq_list &list, int64_t *n_tiles)
+{
+    if (a.B == 1) {
+        const vx_kvq_seq s = vx_kvq_request(a, 0);
+        *n_tiles = (s.nq + QT - 1) / QT * a.n_kv;
+        return *n_tiles * vx_kvq_weight(s);
+    }
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int b0, b1, tiles = 0;
+    vx_kvq_run(a, &b0, &b1);
+    int64_t mine = 0;
+    for (int b = b0; b < b1; b++) {
+        const vx_kvq_seq s = vx_kvq_request(a, b);
+        const int t = (s.nq + QT - 1) / QT * a.n_kv;
+        mine += (int64_t)t * vx_kvq_weight(s);
+        tiles += t;
+        list.one[tid] = s;
+    }
+    int64_t at = mine;
+    for (int o = 1; o < 64; o <<= 1) {
+        const int64_t u = __shfl_up(at, o);
+        const int t = __shfl_up(tiles, o);
+        if (lane >= o) {
+            at += u;
+            tiles += t;
+        }
+    }
+    if (lane == 63) {
+        list.wave[wave] = at;
+        list.tiles[wave] = tiles;
+    }
+    __syncthreads();
+    int64_t total = 0, nt = 0;
+    for (int w = 0; w < AK_WAVES; w++) {
+        if (w < wave) at += list.wave[w];
+        total += list.wave[w];
+        nt += list.tiles[w];
+    }
+    list.at[tid + 1] = at;
+    if (tid == 0) list.at[0] = 0;
+    __syncthreads();
+    *n_tiles = vx_uniform(nt);
+    return vx_uniform(total);
+}
+
+// What stands at item x of request b, whose items begin at base.
+__device__ __forceinline__ vx_kvq_found vx_kvq_place(const vx_kvq_seq &s, int b, int64_t base, int64_t x)
+{
+    vx_kvq_found f;
+    const int w = vx_kvq_weight(s);
+    f.s = s;
+    f.b = b;
+    f.nth = (int)vx_quot(x - base, w);
+    f.first = base + (int64_t)f.nth * w;
+    return f;
+}
+
+// The thread whose run holds item x writes what is there to list.found[k]
+// (of one request, each thread finds it by itself: vx_kvq_get).
+template <int QT>
+__device__ __forceinline__ void vx_kvq_find(const vx_kvq_batch &a, vx_kvq_list &list, int64_t x, int k)
+{
+    if (a.B == 1) return;
+    const int tid = threadIdx.x;
+    int64_t base = list.at[tid];
+    if (x < base || x >= list.at[tid + 1]) return;
+    int b0, b1;
+    vx_kvq_run(a, &b0, &b1);
+    for (int b = b0; b < b1; b++) {
+        const vx_kvq_seq s = b1 - b0 == 1 ? list.one[tid] : vx_kvq_request(a, b);
+        const int64_t w = (int64_t)((s.nq + QT - 1) / QT) * vx_kvq_weight(s) * a.n_kv;
+        if (x < base + w) {
+            list.found[k] = vx_kvq_place(s, b, base, x);
+            return;
+        }
+        base += w;
+    }
+}
+
+// The same in every thread, behind a barrier, in scalar registers.
+__device__ __forceinline__ vx_kvq_found vx_kvq_get(const vx_kvq_batch &a, const vx_kvq_list &list, int64_t x, int k)
+{
+    if (a.B == 1) return vx_kvq_place(vx_kvq_request(a, 0), 0, 0, x);
+    vx_kvq_found f;
+    f.s.row = __builtin_amdgcn_readfirstlane(list.found[k].s.row);
+    f.s.m = __builtin_amdgcn_readfirstlane(list.found[k].s.m);
+    f.s.n = __builtin_amdgcn_readfirstlane(list.found[k].s.n);
+    f.s.end = __builtin_amdgcn_readfirstlane(list.found[k].s.end);
+    f.s.nq = f.s.m * a.G;
+    f.b = __builtin_amdgcn_readfirstlane(list.found[k].b);
+    f.nth = __builtin_amdgcn_readfirstlane(list.found[k].nth);
+    f.first = vx_uniform(list.found[k].first);
+    return f;
+}
+
+// Boundary y of two pieces, moved to an end of its tile when that is near.
+__device__ __forceinline__ int64_t vx_kvq_snap(const vx_kvq_found &f, int64_t y, int snap)
+{
+    const int64_t end = f.first + vx_kvq_weight(f.s);
+    return y - f.first <= snap + AK_BEGIN ? f.first : end - y <= snap ? end : y;
+}
+
+// Counts the workgroup in after its partial results have reached memory;
+// true for the last of n, which sets the counter back.
+__device__ __forceinline__ bool vx_arrive(unsigned *counter, int n, unsigned *s_last)
+{
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        *s_last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (*s_last == (unsigned)(n - 1)) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    return *s_last == (unsigned)(n - 1);
+}
+
+// Parts i0..i1-1 of nv queries joined, in order, AK_JOIN at a time: their
+// loads wait for memory once.
+template <int HD, int QT, int THREADS, typename Slot, typename Out>
+__device__ __forceinline__ void vx_kvq_join(const float *part, Slot slot, int i0, int i1, int nv, Out put)
+{
+    constexpr int PS = HD + 4;
+    for (int u = threadIdx.x; u < nv * (HD / 4); u += THREADS) {
+        const int qq = u / (HD / 4), d = u % (HD / 4) * 4;
+        float mx = -INFINITY, sum = 0.0f;
+        vx_f32x4 o = vx_f32x4{};
+        for (int p = i0; p < i1; p += AK_JOIN) {
+            float2 ml[AK_JOIN], v0[AK_JOIN], v1[AK_JOIN];
+            float nm = mx;
 #pragma unroll
-    for (int d = 0; d < HD; d++) {
-        const float v = vx_wave_sum64(o[d] * f);
-        if (lane == 0) out[(size_t)r * ld_out + h * HD + d] = l > 0.0f ? v / l : 0.0f;
+            for (int i = 0; i < AK_JOIN; i++) {
+                const float *pp = part + ((size_t)slot(min(p + i, i1 - 1)) * QT + qq) * PS;
+                ml[i] = vx_dev_load2(pp + HD);
+                v0[i] = vx_dev_load2(pp + d);
+                v1[i] = vx_dev_load2(pp + d + 2);
+            }
+#pragma unroll
+            for (int i = 0; i < AK_JOIN; i++) {
+                if (p + i >= i1) ml[i] = make_float2(-INFINITY, 0.0f);
+                nm = fmaxf(nm, ml[i].x);
+            }
+            const float ref = nm == -INFINITY ? 0.0f : nm, fo = __builtin_amdgcn_exp2f(mx - ref);
+            sum *= fo;
+            o *= fo;
+#pragma unroll
+            for (int i = 0; i < AK_JOIN; i++) {
+                const float f = __builtin_amdgcn_exp2f(ml[i].x - ref);
+                sum = fmaf(ml[i].y, f, sum);
+                if (p + i < i1) o += vx_f32x4{v0[i].x, v0[i].y, v1[i].x, v1[i].y} * f;
+            }
+            mx = nm;
+        }
+        put(qq, d, o, mx, sum);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Few queries (decode, verify): bound by the cache's bytes.  Per 32 tokens a
+// wavefront loads K and V straight into MFMA operand order (16 bytes a lane),
+// converts them to fp16 exactly and multiplies 16 NQ queries kept as two fp16
+// parts (22 bits).  S = K Q^T leaves a lane with tokens 4g..4g+3, 16+4g.. of
+// query n, which is the operand P V wants: no exchange between lanes but the
+// maximum's.  The four wavefronts take every fourth group and join in LDS.
+// ---------------------------------------------------------------------------
+template <int TYPE, int HD, int NQ>
+__global__ __launch_bounds__(AK_THREADS, NQ == 1 ? 3 : 2) void vx_attention_kvq_kernel(
+    const float *__restrict__ q, int ldq, vx_kvq_batch a, const int *__restrict__ table, int ld_table,
+    const uint8_t *__restrict__ kc, const uint8_t *__restrict__ vc, const float *__restrict__ ks,
+    const float *__restrict__ vs, int shift, int n_pages, float *__restrict__ out, int ld_out,
+    float *__restrict__ part, unsigned *__restrict__ counter)
+{
+    constexpr int QT = 16 * NQ, NJ = HD / 32, ND = HD / 16, PS = HD + 4;
+    // the queries' operands, [query tile][hi, lo][32 dims][lane]; after the last
+    // group the wavefronts' results, [wave][query][values, maximum, sum]
+    __shared__ union {
+        uint4 q[AK_WAVES][NQ][2][NJ][64];
+        float o[AK_WAVES][QT][PS];
+    } sh;
+    __shared__ vx_kvq_list list;
+    __shared__ unsigned s_last;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15, g4 = lane >> 4;
+
+    int64_t n_tiles;
+    const int64_t total = vx_kvq_scan<QT>(a, list, &n_tiles);
+    if (total == 0) return;
+    // pieces of whole rounds of the wavefronts, and no less than a sixteenth of
+    // an average tile where that is little
+    int64_t piece = vx_quot(total + gridDim.x - 1, gridDim.x);
+    const int64_t part16 = min(max(vx_quot(total + n_tiles * AK_BLOCK - 1, n_tiles * AK_BLOCK), (int64_t)8), (int64_t)24);
+    piece = vx_uniform((max(piece, part16) + AK_WAVES - 1) / AK_WAVES * AK_WAVES);
+    // a boundary this near a tile's end moves there: beginning a tile costs more
+    const int snap = __builtin_amdgcn_readfirstlane((int)min(piece / 4, (int64_t)AK_SNAP));
+    const int64_t start = (int64_t)blockIdx.x * piece;
+    if (start >= total) return;
+    vx_kvq_find<QT>(a, list, start, 0);
+    vx_kvq_find<QT>(a, list, start + piece, 1);
+    __syncthreads();
+    int64_t w_end = total;
+    if (start + piece < total) w_end = vx_kvq_snap(vx_kvq_get(a, list, start + piece, 1), start + piece, snap);
+    int64_t x = vx_kvq_snap(vx_kvq_get(a, list, start, 0), start, snap);
+    if (x != start && x < w_end) {
+        __syncthreads();
+        vx_kvq_find<QT>(a, list, x, 0);
+        __syncthreads();
+    }
+
+    while (x < w_end) {
+        const vx_kvq_found f = vx_kvq_get(a, list, x, 0);
+        const vx_kvq_seq s = f.s;
+        const int b = f.b, groups = vx_kvq_groups(s), tiles = (s.nq + QT - 1) / QT;
+        const int64_t first = f.first;                        // the tile's items: [first, first + weight)
+        const int g_begin = max((int)(x - first) - AK_BEGIN, 0);
+        const int g_end = (int)min((int64_t)groups, w_end - first - AK_BEGIN);
+        // short tiles of one request: a wavefront each
+        int few = 1;
+        if (groups <= AK_SMALL && g_begin == 0 && g_end == groups)
+            few = min(min(AK_WAVES, tiles * a.n_kv - f.nth), (int)vx_quot(w_end - first, groups + AK_BEGIN));
+        const int nth = f.nth + (few > 1 ? min(wave, few - 1) : 0), kvh = nth / tiles, tile = nth % tiles;
+        const int stride = few > 1 ? 1 : AK_WAVES, qw = few > 1 ? wave : 0;
+
+        const int q0 = tile * QT;
+        // what every query of the tile reads, and what none passes
+        int lo = s.n - s.m + q0 / a.G + 1, hi = s.n - s.m + min(q0 + QT - 1, s.nq - 1) / a.G + 1;
+        if (a.cap > 0) {
+            lo = min(lo, a.cap);
+            hi = min(hi, a.cap);
+        }
+
+        // queries: hi and lo parts (each wavefront stores some dims), positions
+        float qs[NQ];
+        int lim[NQ];
+        float4 x0[NQ][NJ], x1[NQ][NJ];
+#pragma unroll
+        for (int i = 0; i < NQ; i++) {
+            const int qi = q0 + 16 * i + n;
+            const bool ok = qi < s.nq;
+            const int row = ok ? qi / a.G : 0;
+            const float *qr = q + (size_t)(s.row + row) * ldq + (size_t)(kvh * a.G + (ok ? qi % a.G : 0)) * HD + 8 * g4;
+            lim[i] = ok ? s.n - s.m + row + 1 : 0x7FFFFFFF;     // a query that is none: any value will do
+            if (a.cap > 0 && ok) lim[i] = min(lim[i], a.cap);
+            qs[i] = ok ? 1.44269504088896340736f / 16384.0f / sqrtf((float)HD) : 0.0f;   // scores in powers of two
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
+                x0[i][j] = *(const float4 *)(qr + 32 * j);
+                x1[i][j] = *(const float4 *)(qr + 32 * j + 4);
+            }
+        }
+        const int pgs = shift - 5;                            // groups of a page, as a shift
+        const int g_stop = few > 1 && wave >= few ? 0 : min(g_end, (hi + 31) >> 5);
+        // the page and the byte of a group's keys and values; page -1: none
+        auto locate = [&](int g, size_t *base) {
+            int page = table[(size_t)b * ld_table + (g >> pgs)];
+            if ((unsigned)page >= (unsigned)n_pages) page = -1;
+            *base = ((((size_t)max(page, 0) * a.n_kv + kvh) << shift) + (size_t)(g & ((1 << pgs) - 1)) * 32) * HD;
+            return page;
+        };
+        uint4 kr[NJ], vr[NJ];
+        int g = few > 1 ? 0 : g_begin + wave, page = -1;
+        if (g < g_stop) {
+            size_t base;
+            page = locate(g, &base);
+#pragma unroll
+            for (int j = 0; j < NJ; j++) kr[j] = *(const uint4 *)(kc + base + lane * 16 + 1024 * j);
+#pragma unroll
+            for (int j = 0; j < NJ; j++) vr[j] = *(const uint4 *)(vc + base + lane * 16 + 1024 * j);
+        }
+
+#pragma unroll
+        for (int i = 0; i < NQ; i++) {
+            float amax = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
+                amax = fmaxf(amax, fmaxf(fmaxf(fabsf(x0[i][j].x), fabsf(x0[i][j].y)), fmaxf(fabsf(x0[i][j].z), fabsf(x0[i][j].w))));
+                amax = fmaxf(amax, fmaxf(fmaxf(fabsf(x1[i][j].x), fabsf(x1[i][j].y)), fmaxf(fabsf(x1[i][j].z), fabsf(x1[i][j].w))));
+            }
+            amax = vx_max_x32(vx_max_x16(amax));
+            // below 2^14, so that the low parts stay normal numbers for long
+            float rs;
+            const float f = vx_row_scale(amax, &rs) * 16384.0f;
+            qs[i] *= rs;
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
+                if (few == 1 && (i * NJ + j) % AK_WAVES != wave) continue;
+                vx_half2 h[4], l[4];
+                vx_split(x0[i][j].x * f, x0[i][j].y * f, &h[0], &l[0]);
+                vx_split(x0[i][j].z * f, x0[i][j].w * f, &h[1], &l[1]);
+                vx_split(x1[i][j].x * f, x1[i][j].y * f, &h[2], &l[2]);
+                vx_split(x1[i][j].z * f, x1[i][j].w * f, &h[3], &l[3]);
+                sh.q[qw][i][0][j][lane] = *(const uint4 *)h;
+                sh.q[qw][i][1][j][lane] = *(const uint4 *)l;
+            }
+        }
+        __syncthreads();
+        vx_f32x4 O[NQ][ND];
+        float m[NQ], l[NQ];
+#pragma unroll
+        for (int i = 0; i < NQ; i++) {
+            m[i] = -INFINITY;
+            l[i] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < ND; d++) O[i][d] = vx_f32x4{};
+        }
+        for (; g < g_stop; g += stride) {
+            // the next group's loads go out as this one's registers come free
+            const bool more = g + stride < g_stop;
+            size_t base;
+            const int next = locate(more ? g + stride : g, &base);
+            const uint8_t *kn = kc + base + lane * 16, *vn = vc + base + lane * 16;
+            const size_t hp = (size_t)max(page, 0) * a.n_kv + kvh;
+            const bool none = page < 0;
+            const float ksc = none ? 0.0f : ks[hp], vsc = none ? 0.0f : vs[hp];
+            page = next;
+            vx_f32x4 S[NQ][2];
+            {
+                // the parts' sums meet at the end: the small ones round by themselves
+                vx_f32x4 L[NQ][2];
+#pragma unroll
+                for (int j = 0; j < NJ; j++) {
+                    const vx_half8 k0 = vx_kvq_half8<TYPE>(kr[j].x, kr[j].y), k1 = vx_kvq_half8<TYPE>(kr[j].z, kr[j].w);
+                    kr[j] = *(const uint4 *)(kn + 1024 * j);
+#pragma unroll
+                    for (int i = 0; i < NQ; i++) {
+                        const vx_half8 qh = __builtin_bit_cast(vx_half8, sh.q[qw][i][0][j][lane]);
+                        const vx_half8 ql = __builtin_bit_cast(vx_half8, sh.q[qw][i][1][j][lane]);
+                        S[i][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qh, j ? S[i][0] : vx_f32x4{}, 0, 0, 0);
+                        S[i][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qh, j ? S[i][1] : vx_f32x4{}, 0, 0, 0);
+                        L[i][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, ql, j ? L[i][0] : vx_f32x4{}, 0, 0, 0);
+                        L[i][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, ql, j ? L[i][1] : vx_f32x4{}, 0, 0, 0);
+                        AK_KEEP(S[i][0], k0, qh);
+                        AK_KEEP(S[i][1], k1, qh);
+                        AK_KEEP(L[i][0], k0, ql);
+                        AK_KEEP(L[i][1], k1, ql);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < NQ; i++) {
+                    S[i][0] += L[i][0];
+                    S[i][1] += L[i][1];
+                }
+            }
+            const int t0 = 32 * g + 4 * g4;
+            vx_half8 ph[NQ], pl[NQ];
+#pragma unroll
+            for (int i = 0; i < NQ; i++) {
+                if (32 * g + 32 > lo || none) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (none || t0 + (e >> 2) * 16 + (e & 3) >= lim[i]) S[i][e >> 2][e & 3] = -INFINITY;
+                }
+                // a scale of zero: -inf must not meet a zero
+                const float c = fmaxf(qs[i] * ksc, 1e-37f);
+                float cm = fmaxf(fmaxf(fmaxf(S[i][0][0], S[i][0][1]), fmaxf(S[i][0][2], S[i][0][3])),
+                                 fmaxf(fmaxf(S[i][1][0], S[i][1][1]), fmaxf(S[i][1][2], S[i][1][3])));
+                cm = vx_max_x32(vx_max_x16(cm)) * c;
+                const float nm = fmaxf(m[i], cm), ref = nm == -INFINITY ? 0.0f : nm;
+                if (__any(nm > m[i])) {
+                    const float f = __builtin_amdgcn_exp2f(m[i] - ref);
+                    l[i] *= f;
+#pragma unroll
+                    for (int d = 0; d < ND; d++) O[i][d] *= f;
+                    m[i] = nm;
+                }
+                // probabilities times 2^14: their low parts stay normal numbers
+                const float sub = 14.0f - ref;
+                float p[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    p[e] = __builtin_amdgcn_exp2f(fmaf(S[i][e >> 2][e & 3], c, sub));
+                    l[i] += p[e];
+                }
+                vx_half2 h[4], w[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) vx_split(p[2 * e], p[2 * e + 1], &h[e], &w[e]);
+                ph[i] = vx_half8{h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
+                pl[i] = vx_half8{w[0][0], w[0][1], w[1][0], w[1][1], w[2][0], w[2][1], w[3][0], w[3][1]};
+            }
+            if (TYPE == VXH_KVQ_E4M3 && (none || 32 * g + 32 > hi)) {
+                // codes that no query reads may be NaN, and 0 times it is
+                uint32_t mk[2] = {0, 0};
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (!none && t0 + (e >> 2) * 16 + (e & 3) < hi) mk[e >> 2] |= 0xFFu << (8 * (e & 3));
+#pragma unroll
+                for (int j = 0; j < NJ; j++)
+                    vr[j] = make_uint4(vr[j].x & mk[0], vr[j].y & mk[1], vr[j].z & mk[0], vr[j].w & mk[1]);
+            }
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
+                const vx_half8 v0 = vx_kvq_half8<TYPE>(vr[j].x, vr[j].y), v1 = vx_kvq_half8<TYPE>(vr[j].z, vr[j].w);
+                vr[j] = *(const uint4 *)(vn + 1024 * j);
+#pragma unroll
+                for (int i = 0; i < NQ; i++) {
+                    vx_f32x4 t = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl[i], vx_f32x4{}, 0, 0, 0);
+                    vx_f32x4 u = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl[i], vx_f32x4{}, 0, 0, 0);
+                    AK_KEEP(t, v0, pl[i]);
+                    AK_KEEP(u, v1, pl[i]);
+                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph[i], t, 0, 0, 0);
+                    u = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph[i], u, 0, 0, 0);
+                    AK_KEEP(t, v0, ph[i]);
+                    AK_KEEP(u, v1, ph[i]);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        O[i][2 * j][e] = fmaf(t[e], vsc, O[i][2 * j][e]);
+                        O[i][2 * j + 1][e] = fmaf(u[e], vsc, O[i][2 * j + 1][e]);
+                    }
+                }
+            }
+        }
+
+        auto finish = [&](int qi, int d, vx_f32x4 o, float sum) {
+            const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+            *(vx_f32x4 *)(out + (size_t)(s.row + qi / a.G) * ld_out + (size_t)(kvh * a.G + qi % a.G) * HD + d) = o * inv;
+        };
+#pragma unroll
+        for (int i = 0; i < NQ; i++) l[i] = vx_sum_x32(vx_sum_x16(l[i]));
+        if (few > 1) {
+#pragma unroll
+            for (int i = 0; i < NQ; i++)
+                if (wave < few && q0 + 16 * i + n < s.nq)
+#pragma unroll
+                    for (int d = 0; d < ND; d++) finish(q0 + 16 * i + n, 16 * d + 4 * g4, O[i][d], l[i]);
+            x = first + (int64_t)few * (groups + AK_BEGIN);
+            __syncthreads();
+            if (x < w_end) {
+                vx_kvq_find<QT>(a, list, x, 0);
+                __syncthreads();
+            }
+            continue;
+        }
+        // the wavefronts' parts meet in LDS
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NQ; i++) {
+            float *so = sh.o[wave][16 * i + n];
+#pragma unroll
+            for (int d = 0; d < ND; d++) *(vx_f32x4 *)(so + 16 * d + 4 * g4) = O[i][d];
+            if (g4 == 0) {
+                so[HD] = m[i];
+                so[HD + 1] = l[i];
+            }
+        }
+        __syncthreads();
+        const bool whole = g_begin == 0 && g_end == groups;
+        // a piece holds at most one tile begun before it and one that goes on behind it
+        float *mine_p = part + (size_t)(2 * blockIdx.x + (g_begin == 0)) * QT * PS;
+        const int nv = min(QT, s.nq - q0);
+        for (int u = tid; u < nv * (HD / 4); u += AK_THREADS) {
+            const int qq = u / (HD / 4), d = u % (HD / 4) * 4;
+            float mx = sh.o[0][qq][HD];
+#pragma unroll
+            for (int w = 1; w < AK_WAVES; w++) mx = fmaxf(mx, sh.o[w][qq][HD]);
+            const float ref = mx == -INFINITY ? 0.0f : mx;
+            float sum = 0.0f;
+            vx_f32x4 o = vx_f32x4{};
+#pragma unroll
+            for (int w = 0; w < AK_WAVES; w++) {
+                const float f = __builtin_amdgcn_exp2f(sh.o[w][qq][HD] - ref);
+                sum = fmaf(sh.o[w][qq][HD + 1], f, sum);
+                o += *(const vx_f32x4 *)(&sh.o[w][qq][d]) * f;
+            }
+            if (whole)
+                finish(q0 + qq, d, o, sum);
+            else {
+                float *pp = mine_p + (size_t)qq * PS;
+#pragma unroll
+                for (int e = 0; e < 4; e += 2) vx_dev_store2(pp + d + e, o[e], o[e + 1]);
+                if (d == 0) vx_dev_store2(pp + HD, mx, sum);
+            }
+        }
+        if (!whole) {
+            // the pieces p0..p1 that hold a part of this tile join in blocks of
+            // AK_BLOCK, and the blocks: each time the last one to finish does it
+            // (its inner boundaries lie past first + AK_BEGIN + snap and before end - snap)
+            const int p0 = (int)vx_quot(first + AK_BEGIN + snap, piece);
+            const int p1 = max((int)vx_quot(first + AK_BEGIN + groups - snap + piece - 1, piece) - 1, p0);
+            const int me = (int)blockIdx.x - p0, blk = me / AK_BLOCK, n_blk = (p1 - p0) / AK_BLOCK + 1;
+            const int c0 = blk * AK_BLOCK, c1 = min(c0 + AK_BLOCK, p1 - p0 + 1);
+            // a piece inside the tile has a second slot: a block's joint result goes
+            // to its first piece's (the first block's to its second, the first may
+            // hold the end of another tile)
+            auto slot0 = [&](int i) { return 2 * (p0 + i) + (i == 0); };
+            auto slot1 = [&](int i) {
+                const int f = i * AK_BLOCK;
+                return f == p1 - p0 ? slot0(f) : 2 * (p0 + f + (i == 0)) + 1;
+            };
+            bool last = c1 - c0 == 1 || vx_arrive(counter + p0 + blk, c1 - c0, &s_last);
+            if (last && n_blk > 1) {
+                if (c1 - c0 > 1)
+                    vx_kvq_join<HD, QT, AK_THREADS>(part, slot0, c0, c1, nv, [&](int qq, int d, vx_f32x4 o, float mx, float sum) {
+                        float *pp = part + ((size_t)slot1(blk) * QT + qq) * PS;
+                        vx_dev_store2(pp + d, o[0], o[1]);
+                        vx_dev_store2(pp + d + 2, o[2], o[3]);
+                        if (d == 0) vx_dev_store2(pp + HD, mx, sum);
+                    });
+                last = vx_arrive(counter + AK_WG + p0, n_blk, &s_last);
+            }
+            auto put = [&](int qq, int d, vx_f32x4 o, float mx, float sum) { finish(q0 + qq, d, o, sum); };
+            if (last && n_blk > 1) vx_kvq_join<HD, QT, AK_THREADS>(part, slot1, 0, n_blk, nv, put);
+            else if (last) vx_kvq_join<HD, QT, AK_THREADS>(part, slot0, 0, c1, nv, put);
+        }
+        x = first + AK_BEGIN + g_end;
+        if (x < w_end) {
+            __syncthreads();
+            vx_kvq_find<QT>(a, list, x, 0);
+            __syncthreads();
+        }
     }
 }
 
 extern "C" size_t vxh_attention_kvq_workspace_floats(int max_rows, int n_seqs, int n_heads, int n_kv_heads,
                                                      int head_dim)
 {
-    return 64;
+    return (size_t)2 * AK_WG * 16 * (head_dim + 4);
 }
 
 extern "C" int vxh_attention_kvq(const float *q, int ldq, const int *row0, const int *len, int n_seqs, int max_rows,
@@ -59,21 +654,35 @@ extern "C" int vxh_attention_kvq(const float *q, int ldq, const int *row0, const
 {
     if (const char *bad = vx_kvq_bad(c)) return vxh_fail(VXH_ERR_PARAM, "attention_kvq: %s", bad);
     const int w = n_heads * c->head_dim;
-    if (!q || !row0 || !len || !table || !out || !ws || n_seqs < 1 || n_seqs > VXH_PAGE_MAX_SEQS || max_rows < 1 ||
-        max_rows > VXH_PAGE_MAX_ROWS || max_seq_rows < 1 || ld_table < 1 || cap < 0 || n_heads < 1 ||
-        n_heads % c->n_kv_heads || ldq < w || ldq % 4 || ld_out < w || ld_out % 4 || ((uintptr_t)q & 15) || ((uintptr_t)out & 15))
+    if (!q || !row0 || !len || !table || !out || !ws || !ws->acc || !ws->part || n_seqs < 1 || n_seqs > VXH_PAGE_MAX_SEQS ||
+        max_rows < 1 || max_rows > VXH_PAGE_MAX_ROWS || max_seq_rows < 1 || ld_table < 1 || cap < 0 || n_heads < 1 ||
+        n_heads % c->n_kv_heads || ldq < w || ldq % 4 || ld_out < w || ld_out % 4 || ((uintptr_t)q & 15) ||
+        ((uintptr_t)out & 15) ||
+        ws->part_floats < vxh_attention_kvq_workspace_floats(max_rows, n_seqs, n_heads, c->n_kv_heads, c->head_dim))
         return vxh_fail(VXH_ERR_PARAM, "attention_kvq: %d requests, %d rows, %d/%d heads of %d (ld %d, %d)", n_seqs,
                         max_rows, n_heads, c->n_kv_heads, c->head_dim, ldq, ld_out);
-    const dim3 grid(max_rows, n_heads);
-#define VX_CALL(T, HD)                                                                                                \
-    vx_attention_kvq_kernel<T, HD><<<grid, 64, 0, vxh_hs(s)>>>(q, ldq, row0, len, n_seqs, max_rows, table, ld_table,  \
-                                                               n_heads, *c, cap, out, ld_out)
+    vx_kvq_batch a;
+    a.row0 = row0;
+    a.len = len;
+    a.B = n_seqs;
+    a.max_rows = max_rows;
+    a.n_kv = c->n_kv_heads;
+    a.G = n_heads / c->n_kv_heads;
+    a.cap = cap;
+    const int64_t limit = (int64_t)ld_table * c->page;
+    a.limit = limit > 0x7FFFFF00 ? 0x7FFFFF00 : (int)limit;
+    const int shift = c->page == 32 ? 5 : c->page == 64 ? 6 : 7;
+    unsigned *counter = (unsigned *)(ws->acc + ws->acc_elems);
+#define VX_CALL(T, HD, NQ)                                                                                            \
+    vx_attention_kvq_kernel<T, HD, NQ><<<AK_WG, AK_THREADS, 0, vxh_hs(s)>>>(                                           \
+        q, ldq, a, table, ld_table, (const uint8_t *)c->k, (const uint8_t *)c->v, c->ks, c->vs, shift, c->n_pages,    \
+        out, ld_out, ws->part, counter)
 #define VX_HD(T)                                                                                                      \
     switch (c->head_dim) {                                                                                            \
-    case 32: VX_CALL(T, 32); break;                                                                                   \
-    case 64: VX_CALL(T, 64); break;                                                                                   \
-    case 96: VX_CALL(T, 96); break;                                                                                   \
-    default: VX_CALL(T, 128);                                                                                         \
+    case 32: VX_CALL(T, 32, 1); break;                                                                                     \
+    case 64: VX_CALL(T, 64, 1); break;                                                                                     \
+    case 96: VX_CALL(T, 96, 1); break;                                                                                     \
+    default: VX_CALL(T, 128, 1);                                                                                           \
     }
     if (c->type == VXH_KVQ_INT8) {
         VX_HD(VXH_KVQ_INT8)

@@ -34,6 +34,9 @@ typedef float vx_f32x16 __attribute__((ext_vector_type(16)));
 
 static inline hipStream_t vxh_hs(vxh_stream s) { return (hipStream_t)s; }
 
+// Completion counters that vxh_workspace_alloc keeps behind the accumulator.
+#define VX_WS_COUNTERS 1024
+
 // Number of 16-byte panel units per block of 32 columns for M rows:
 // 2 MFMA halves (s) x 2 lane halves (h) x 2M slots.
 static inline int vxh_panel_units_per_block(int M) { return 2 * 2 * 2 * M; }

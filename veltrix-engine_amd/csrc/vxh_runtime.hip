@@ -238,12 +238,15 @@ extern "C" int vxh_graph_destroy(vxh_graph g)
 extern "C" int vxh_workspace_alloc(vxh_workspace *w, size_t acc_elems, size_t part_floats)
 {
     memset(w, 0, sizeof(*w));
-    int rc = vxh_malloc((void **)&w->acc, acc_elems * sizeof(double));
+    // behind the accumulator, the completion counters of the attention over the
+    // paged cache: zeroed with it, left zeroed by every call
+    const size_t acc_bytes = acc_elems * sizeof(double) + VX_WS_COUNTERS * sizeof(unsigned);
+    int rc = vxh_malloc((void **)&w->acc, acc_bytes);
     if (rc) return rc;
     rc = vxh_malloc((void **)&w->part, part_floats * sizeof(float));
     if (rc) { vxh_free(w->acc); w->acc = nullptr; return rc; }
     // the accumulator starts zeroed; every consumer clears what it reads
-    VXH_CHECK(hipMemset(w->acc, 0, acc_elems * sizeof(double)));
+    VXH_CHECK(hipMemset(w->acc, 0, acc_bytes));
     VXH_CHECK(hipDeviceSynchronize());
     w->acc_elems = acc_elems;
     w->part_floats = part_floats;
