@@ -301,6 +301,15 @@ BATCHES = [
     ([140], [140], 16, 1, 32, 32, 64),
     ([3000, 5, 17, 1200], [1, 1, 2, 1], 4, 4, 128, 32, 2049),
     ([40] * 70, [2] * 70, 4, 2, 64, 32, 0),
+    # enough query tiles for the prompt kernel: of four streams, of two
+    ([130], [130], 64, 64, 32, 32, 0),
+    ([1100], [97], 224, 32, 32, 64, 0),
+    ([333], [129], 64, 64, 96, 128, 200),
+    ([2049, 40, 66, 300], [64, 0, 66, 1], 64, 64, 64, 32, 2049),
+    ([70, 400, 5, 31], [65, 300, 1, 31], 64, 64, 64, 64, 0),
+    ([300, 700], [200, 200], 128, 16, 32, 128, 0),
+    ([500], [390], 64, 64, 128, 64, 77),
+    ([90] * 40, [70] * 40, 16, 8, 32, 32, 0),
 ]
 
 
@@ -326,11 +335,11 @@ def test_attention(P, kind, case):
 
 
 @pytest.mark.parametrize("kind", [Q.INT8, Q.E4M3])
-@pytest.mark.parametrize("rows", [1, 9, 150])
-def test_attention_ignores_what_no_row_reads(P, kind, rows):
+@pytest.mark.parametrize("rows,H,KV", [(1, 6, 2), (9, 6, 2), (150, 6, 2), (150, 64, 64)])
+def test_attention_ignores_what_no_row_reads(P, kind, rows, H, KV):
     """Bytes of every kind (e4m3 NaN among them) behind the last token, NaN
     scales on pages behind it, garbage in the table's unused columns."""
-    page, KV, H, hd, n = 64, 2, 6, 64, 203
+    page, hd, n = 64, 64, 203
     rng = np.random.default_rng(rows)
     pool, table, row0 = ragged(rng, [n], [rows], page, extra_cols=2)
     dc, oc = filled(P, kind, page, pool, KV, hd, rng)
@@ -362,11 +371,11 @@ def test_attention_ignores_what_no_row_reads(P, kind, rows):
     dc.free()
 
 
-@pytest.mark.parametrize("rows", [1, 5, 140])
-def test_attention_of_lengths_and_tables_that_lie(P, rows):
+@pytest.mark.parametrize("rows,H,KV", [(1, 4, 2), (5, 4, 2), (140, 4, 2), (70, 48, 48)])
+def test_attention_of_lengths_and_tables_that_lie(P, rows, H, KV):
     """Table entries that are no page, lengths past the table, fewer tokens
     than rows, negative lengths: rows read what there is, or are zeros."""
-    page, KV, H, hd = 32, 2, 4, 64
+    page, hd = 32, 64
     rng = np.random.default_rng(rows + 1)
     dc, oc = filled(P, Q.INT8, page, 12, KV, hd, rng)
     table = np.array([[3, -1, 5, 7, 9], [1, 2, 12, 2 ** 31 - 1, 4], [0, 6, 8, 10, 11], [-1, -1, -1, -1, -1]], np.int32)
@@ -383,23 +392,24 @@ def test_attention_of_lengths_and_tables_that_lie(P, rows):
     dc.free()
 
 
-def test_attention_scores_far_apart(P):
+@pytest.mark.parametrize("rows,H,KV", [(3, 2, 1), (66, 96, 96)])
+def test_attention_scores_far_apart(P, rows, H, KV):
     """Scores over a range that underflows every probability but one, large
     and tiny queries, scales that differ by 2^40 between pages."""
-    page, KV, H, hd, n = 32, 1, 2, 64, 1000
+    page, hd, n = 32, 64, 1000 if rows == 3 else 300
     rng = np.random.default_rng(8)
-    pool, table, row0 = ragged(rng, [n], [3], page)
+    pool, table, row0 = ragged(rng, [n], [rows], page)
     for kind in (Q.INT8, Q.E4M3):
         dc, oc = filled(P, kind, page, pool, KV, hd, rng)
         for qs in (1e-30, 40.0, 3000.0):
-            q = (rng.normal(0, 1, (3, H * hd)) * qs).astype(np.float32)
+            q = (rng.normal(0, 1, (rows, H * hd)) * qs).astype(np.float32)
             check_attend(P, dc, oc, q, row0, [n], table, H, 0)
         q[1] = 0
         check_attend(P, dc, oc, q, row0, [n], table, H, 0)
         sc = (2.0 ** rng.integers(-30, 10, (pool, KV))).astype(np.float32)
         oc.scale[1] = sc
         assert P.vxh_upload(C.c_void_p(dc.s.vs), N._ptr(sc), sc.nbytes, None) == 0
-        check_attend(P, dc, oc, rng.normal(0, 1, (3, H * hd)).astype(np.float32), row0, [n], table, H, 0)
+        check_attend(P, dc, oc, rng.normal(0, 1, (rows, H * hd)).astype(np.float32), row0, [n], table, H, 0)
         dc.free()
 
 

@@ -1,89 +1,29 @@
-// Attention of a ragged batch over the paged 8-bit KV cache.
+// Attention of a ragged batch over the paged 8-bit KV cache: the entry point,
+// and the kernel of requests with few queries (decode, verify).
 //
 // A request's rows and the G = n_heads / n_kv_heads query heads of one kv head
-// make up its queries there (query i: row i / G, head i % G), taken in tiles.
-// The work is the list of all (request, kv head, tile, 32-token group); every
-// workgroup takes an equal, consecutive piece of it, so lengths may differ as
-// they like: a long request spreads over many workgroups, short ones share
-// one.  A tile cut by a piece's ends leaves partial results (maximum, sum,
-// weighted values) in the workspace, joined in order by the last workgroup
-// that contributes to it.
-#include "vxh_kvq.h"
-
-typedef float vx_f32x4 __attribute__((ext_vector_type(4)));
+// make up its queries there (query i: row i / G, head i % G), taken 16 to a
+// tile.  The work is the list of all (request, kv head, tile, 32-token group);
+// every workgroup takes an equal, consecutive piece of it, so lengths may
+// differ as they like: a long request spreads over many workgroups, short ones
+// share one.  A tile cut by a piece's ends leaves partial results (maximum,
+// sum, weighted values) in the workspace, joined in order by the last
+// workgroup that contributes to it.
+#include "vxh_attn_kvq.h"
 
 #define AK_WAVES 4
 #define AK_THREADS (64 * AK_WAVES)
 #define AK_WG 512                // pieces: two workgroups per CU
 #define AK_BEGIN 8               // what beginning and ending a tile costs, in 32-token groups
 #define AK_SMALL 8               // tiles of up to this many groups take a wavefront each
+#define AK_SNAP 12               // most groups a piece's end moves to a tile's
+#define AK_FEW 64                // queries per kv head up to which a request is this kernel's
 #define AK_JOIN 8                // parts whose loads are in flight together
 #define AK_BLOCK 16              // parts one workgroup joins
-#define AK_SNAP 12
-
-// ---------------------------------------------------------------------------
-// The work list.  Every workgroup counts it anew from the lengths (they are on
-// the device only): a thread sums a run of requests, the runs are scanned.
-// ---------------------------------------------------------------------------
-struct vx_kvq_batch {
-    const int *row0, *len;
-    int B, max_rows, n_kv, G, cap, limit;    // limit: tokens a table row can name
-};
-
-struct vx_kvq_seq {
-    int row, m, n, end, nq;      // first row, rows, tokens, tokens any row reads, queries per kv head
-};
-
-__device__ __forceinline__ vx_kvq_seq vx_kvq_request(const vx_kvq_batch &a, int b)
-{
-    vx_kvq_seq s;
-    s.row = min(max(a.row0[b], 0), a.max_rows);
-    s.m = max(min(a.row0[b + 1], a.max_rows) - s.row, 0);
-    s.n = min(max(a.len[b], 0), a.limit);
-    s.end = a.cap > 0 ? min(s.n, a.cap) : s.n;
-    s.nq = s.m * a.G;
-    return s;
-}
-
-// 32-token groups of every tile of one kv head (at least one: a tile that
-// reads nothing still writes its zeros).
-__device__ __forceinline__ int vx_kvq_groups(const vx_kvq_seq &s) { return max((s.end + 31) >> 5, 1); }
 
 // Items of a tile: its groups, behind AK_BEGIN that stand for what beginning
 // and ending a tile cost.
 __device__ __forceinline__ int vx_kvq_weight(const vx_kvq_seq &s) { return vx_kvq_groups(s) + AK_BEGIN; }
-
-// 8 codes to fp16, exactly.
-template <int TYPE>
-__device__ __forceinline__ vx_half8 vx_kvq_half8(uint32_t a, uint32_t b)
-{
-    vx_half2 h[4];
-    if (TYPE == VXH_KVQ_INT8) {
-        // 0x64xx is 1024 + xx
-        const vx_half2 off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
-        h[0] = __builtin_bit_cast(vx_half2, __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u)) + off;
-        h[1] = __builtin_bit_cast(vx_half2, __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u)) + off;
-        h[2] = __builtin_bit_cast(vx_half2, __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u)) + off;
-        h[3] = __builtin_bit_cast(vx_half2, __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)) + off;
-    } else {
-        h[0] = __builtin_bit_cast(vx_half2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, false));
-        h[1] = __builtin_bit_cast(vx_half2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, true));
-        h[2] = __builtin_bit_cast(vx_half2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, false));
-        h[3] = __builtin_bit_cast(vx_half2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, true));
-    }
-    return vx_half8{h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
-}
-
-// x = hi + lo to 22 bits (both truncated, so the two add up with one sign).
-__device__ __forceinline__ void vx_split(float a, float b, vx_half2 *hi, vx_half2 *lo)
-{
-    *hi = __builtin_bit_cast(vx_half2, __builtin_amdgcn_cvt_pkrtz(a, b));
-    *lo = __builtin_bit_cast(vx_half2, __builtin_amdgcn_cvt_pkrtz(a - (float)(*hi)[0], b - (float)(*hi)[1]));
-}
-
-// MFMA sources stay live past the instruction: a destination in VGPRs that
-// overlaps them gives wrong values.
-#define AK_KEEP(D, A, B) asm("" : "+v"(D) : "v"(A), "v"(B))
 
 __device__ __forceinline__ void vx_dev_store2(float *p, float a, float b)
 {
@@ -115,6 +55,8 @@ struct vx_kvq_found {
     int64_t first;
 };
 
+// The list, counted anew by every workgroup from the lengths (they are on the
+// device only): a thread sums a run of requests, the runs are scanned.
 struct vx_kvq_list {
     int64_t at[AK_THREADS + 1];      // items before each thread's run of requests
     vx_kvq_seq one[AK_THREADS];      // a run's last request (its only one up to AK_THREADS requests)
@@ -131,12 +73,11 @@ __device__ __forceinline__ void vx_kvq_run(const vx_kvq_batch &a, int *b0, int *
 }
 
 // Items of the whole list.
-template <int QT>
 __device__ __forceinline__ int64_t vx_kvq_scan(const vx_kvq_batch &a, vx_kvq_list &list, int64_t *n_tiles)
 {
     if (a.B == 1) {
-        const vx_kvq_seq s = vx_kvq_request(a, 0);
-        *n_tiles = (s.nq + QT - 1) / QT * a.n_kv;
+        const vx_kvq_seq s = vx_kvq_request<false>(a, 0);
+        *n_tiles = (s.nq + 15) / 16 * a.n_kv;
         return *n_tiles * vx_kvq_weight(s);
     }
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -144,8 +85,8 @@ __device__ __forceinline__ int64_t vx_kvq_scan(const vx_kvq_batch &a, vx_kvq_lis
     vx_kvq_run(a, &b0, &b1);
     int64_t mine = 0;
     for (int b = b0; b < b1; b++) {
-        const vx_kvq_seq s = vx_kvq_request(a, b);
-        const int t = (s.nq + QT - 1) / QT * a.n_kv;
+        const vx_kvq_seq s = vx_kvq_request<false>(a, b);
+        const int t = (s.nq + 15) / 16 * a.n_kv;
         mine += (int64_t)t * vx_kvq_weight(s);
         tiles += t;
         list.one[tid] = s;
@@ -191,7 +132,6 @@ __device__ __forceinline__ vx_kvq_found vx_kvq_place(const vx_kvq_seq &s, int b,
 
 // The thread whose run holds item x writes what is there to list.found[k]
 // (of one request, each thread finds it by itself: vx_kvq_get).
-template <int QT>
 __device__ __forceinline__ void vx_kvq_find(const vx_kvq_batch &a, vx_kvq_list &list, int64_t x, int k)
 {
     if (a.B == 1) return;
@@ -201,8 +141,8 @@ __device__ __forceinline__ void vx_kvq_find(const vx_kvq_batch &a, vx_kvq_list &
     int b0, b1;
     vx_kvq_run(a, &b0, &b1);
     for (int b = b0; b < b1; b++) {
-        const vx_kvq_seq s = b1 - b0 == 1 ? list.one[tid] : vx_kvq_request(a, b);
-        const int64_t w = (int64_t)((s.nq + QT - 1) / QT) * vx_kvq_weight(s) * a.n_kv;
+        const vx_kvq_seq s = b1 - b0 == 1 ? list.one[tid] : vx_kvq_request<false>(a, b);
+        const int64_t w = (int64_t)((s.nq + 15) / 16) * vx_kvq_weight(s) * a.n_kv;
         if (x < base + w) {
             list.found[k] = vx_kvq_place(s, b, base, x);
             return;
@@ -214,7 +154,7 @@ __device__ __forceinline__ void vx_kvq_find(const vx_kvq_batch &a, vx_kvq_list &
 // The same in every thread, behind a barrier, in scalar registers.
 __device__ __forceinline__ vx_kvq_found vx_kvq_get(const vx_kvq_batch &a, const vx_kvq_list &list, int64_t x, int k)
 {
-    if (a.B == 1) return vx_kvq_place(vx_kvq_request(a, 0), 0, 0, x);
+    if (a.B == 1) return vx_kvq_place(vx_kvq_request<false>(a, 0), 0, 0, x);
     vx_kvq_found f;
     f.s.row = __builtin_amdgcn_readfirstlane(list.found[k].s.row);
     f.s.m = __builtin_amdgcn_readfirstlane(list.found[k].s.m);
@@ -250,11 +190,11 @@ __device__ __forceinline__ bool vx_arrive(unsigned *counter, int n, unsigned *s_
 
 // Parts i0..i1-1 of nv queries joined, in order, AK_JOIN at a time: their
 // loads wait for memory once.
-template <int HD, int QT, int THREADS, typename Slot, typename Out>
+template <int HD, typename Slot, typename Out>
 __device__ __forceinline__ void vx_kvq_join(const float *part, Slot slot, int i0, int i1, int nv, Out put)
 {
     constexpr int PS = HD + 4;
-    for (int u = threadIdx.x; u < nv * (HD / 4); u += THREADS) {
+    for (int u = threadIdx.x; u < nv * (HD / 4); u += AK_THREADS) {
         const int qq = u / (HD / 4), d = u % (HD / 4) * 4;
         float mx = -INFINITY, sum = 0.0f;
         vx_f32x4 o = vx_f32x4{};
@@ -263,7 +203,7 @@ __device__ __forceinline__ void vx_kvq_join(const float *part, Slot slot, int i0
             float nm = mx;
 #pragma unroll
             for (int i = 0; i < AK_JOIN; i++) {
-                const float *pp = part + ((size_t)slot(min(p + i, i1 - 1)) * QT + qq) * PS;
+                const float *pp = part + ((size_t)slot(min(p + i, i1 - 1)) * 16 + qq) * PS;
                 ml[i] = vx_dev_load2(pp + HD);
                 v0[i] = vx_dev_load2(pp + d);
                 v1[i] = vx_dev_load2(pp + d + 2);
@@ -289,34 +229,34 @@ __device__ __forceinline__ void vx_kvq_join(const float *part, Slot slot, int i0
 }
 
 // ---------------------------------------------------------------------------
-// Few queries (decode, verify): bound by the cache's bytes.  Per 32 tokens a
-// wavefront loads K and V straight into MFMA operand order (16 bytes a lane),
-// converts them to fp16 exactly and multiplies 16 NQ queries kept as two fp16
-// parts (22 bits).  S = K Q^T leaves a lane with tokens 4g..4g+3, 16+4g.. of
-// query n, which is the operand P V wants: no exchange between lanes but the
-// maximum's.  The four wavefronts take every fourth group and join in LDS.
+// Bound by the cache's bytes.  Per 32 tokens a wavefront loads K and V straight
+// into MFMA operand order (16 bytes a lane), converts them to fp16 exactly and
+// multiplies 16 queries kept as two fp16 parts (22 bits).  S = K Q^T leaves a
+// lane with tokens 4g..4g+3, 16+4g.. of query n, which is the operand P V
+// wants: no exchange between lanes but the maximum's.  The four wavefronts take
+// every fourth group and join in LDS; short tiles take a wavefront each.
 // ---------------------------------------------------------------------------
-template <int TYPE, int HD, int NQ>
-__global__ __launch_bounds__(AK_THREADS, NQ == 1 ? 3 : 2) void vx_attention_kvq_kernel(
-    const float *__restrict__ q, int ldq, vx_kvq_batch a, const int *__restrict__ table, int ld_table,
-    const uint8_t *__restrict__ kc, const uint8_t *__restrict__ vc, const float *__restrict__ ks,
-    const float *__restrict__ vs, int shift, int n_pages, float *__restrict__ out, int ld_out,
+template <int TYPE, int HD>
+__global__ __launch_bounds__(AK_THREADS, 3) void vx_attention_kvq_kernel(
+    vx_kvq_call c, const float *__restrict__ q, const int *__restrict__ table, const uint8_t *__restrict__ kc,
+    const uint8_t *__restrict__ vc, const float *__restrict__ ks, const float *__restrict__ vs, float *__restrict__ out,
     float *__restrict__ part, unsigned *__restrict__ counter)
 {
-    constexpr int QT = 16 * NQ, NJ = HD / 32, ND = HD / 16, PS = HD + 4;
-    // the queries' operands, [query tile][hi, lo][32 dims][lane]; after the last
-    // group the wavefronts' results, [wave][query][values, maximum, sum]
+    constexpr int NJ = HD / 32, ND = HD / 16, PS = HD + 4;
+    // the queries' operands, [tile][hi, lo][32 dims][lane]; after the last group
+    // the wavefronts' results, [wave][query][values, maximum, sum]
     __shared__ union {
-        uint4 q[AK_WAVES][NQ][2][NJ][64];
-        float o[AK_WAVES][QT][PS];
+        uint4 q[AK_WAVES][2][NJ][64];
+        float o[AK_WAVES][16][PS];
     } sh;
     __shared__ vx_kvq_list list;
     __shared__ unsigned s_last;
+    const vx_kvq_batch &a = c.a;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, g4 = lane >> 4;
 
     int64_t n_tiles;
-    const int64_t total = vx_kvq_scan<QT>(a, list, &n_tiles);
+    const int64_t total = vx_kvq_scan(a, list, &n_tiles);
     if (total == 0) return;
     // pieces of whole rounds of the wavefronts, and no less than a sixteenth of
     // an average tile where that is little
@@ -327,22 +267,22 @@ __global__ __launch_bounds__(AK_THREADS, NQ == 1 ? 3 : 2) void vx_attention_kvq_
     const int snap = __builtin_amdgcn_readfirstlane((int)min(piece / 4, (int64_t)AK_SNAP));
     const int64_t start = (int64_t)blockIdx.x * piece;
     if (start >= total) return;
-    vx_kvq_find<QT>(a, list, start, 0);
-    vx_kvq_find<QT>(a, list, start + piece, 1);
+    vx_kvq_find(a, list, start, 0);
+    vx_kvq_find(a, list, start + piece, 1);
     __syncthreads();
     int64_t w_end = total;
     if (start + piece < total) w_end = vx_kvq_snap(vx_kvq_get(a, list, start + piece, 1), start + piece, snap);
     int64_t x = vx_kvq_snap(vx_kvq_get(a, list, start, 0), start, snap);
     if (x != start && x < w_end) {
         __syncthreads();
-        vx_kvq_find<QT>(a, list, x, 0);
+        vx_kvq_find(a, list, x, 0);
         __syncthreads();
     }
 
     while (x < w_end) {
         const vx_kvq_found f = vx_kvq_get(a, list, x, 0);
         const vx_kvq_seq s = f.s;
-        const int b = f.b, groups = vx_kvq_groups(s), tiles = (s.nq + QT - 1) / QT;
+        const int b = f.b, groups = vx_kvq_groups(s), tiles = (s.nq + 15) / 16;
         const int64_t first = f.first;                        // the tile's items: [first, first + weight)
         const int g_begin = max((int)(x - first) - AK_BEGIN, 0);
         const int g_end = (int)min((int64_t)groups, w_end - first - AK_BEGIN);
@@ -353,40 +293,22 @@ __global__ __launch_bounds__(AK_THREADS, NQ == 1 ? 3 : 2) void vx_attention_kvq_
         const int nth = f.nth + (few > 1 ? min(wave, few - 1) : 0), kvh = nth / tiles, tile = nth % tiles;
         const int stride = few > 1 ? 1 : AK_WAVES, qw = few > 1 ? wave : 0;
 
-        const int q0 = tile * QT;
+        const int q0 = 16 * tile;
         // what every query of the tile reads, and what none passes
-        int lo = s.n - s.m + q0 / a.G + 1, hi = s.n - s.m + min(q0 + QT - 1, s.nq - 1) / a.G + 1;
-        if (a.cap > 0) {
-            lo = min(lo, a.cap);
-            hi = min(hi, a.cap);
-        }
+        const int lo = vx_kvq_limit(a, s, q0), hi = vx_kvq_limit(a, s, min(q0 + 15, s.nq - 1));
+        const int qi = q0 + n;
+        const bool ok = qi < s.nq;
+        const int lim = ok ? vx_kvq_limit(a, s, qi) : hi;             // (a query that is none sees what the others see)
+        vx_kvq_query<NJ> x0;
+        x0.load(q + (size_t)(s.row + (ok ? qi / a.G : 0)) * c.ldq + (size_t)(kvh * a.G + (ok ? qi % a.G : 0)) * HD + 8 * g4);
 
-        // queries: hi and lo parts (each wavefront stores some dims), positions
-        float qs[NQ];
-        int lim[NQ];
-        float4 x0[NQ][NJ], x1[NQ][NJ];
-#pragma unroll
-        for (int i = 0; i < NQ; i++) {
-            const int qi = q0 + 16 * i + n;
-            const bool ok = qi < s.nq;
-            const int row = ok ? qi / a.G : 0;
-            const float *qr = q + (size_t)(s.row + row) * ldq + (size_t)(kvh * a.G + (ok ? qi % a.G : 0)) * HD + 8 * g4;
-            lim[i] = ok ? s.n - s.m + row + 1 : 0x7FFFFFFF;     // a query that is none: any value will do
-            if (a.cap > 0 && ok) lim[i] = min(lim[i], a.cap);
-            qs[i] = ok ? 1.44269504088896340736f / 16384.0f / sqrtf((float)HD) : 0.0f;   // scores in powers of two
-#pragma unroll
-            for (int j = 0; j < NJ; j++) {
-                x0[i][j] = *(const float4 *)(qr + 32 * j);
-                x1[i][j] = *(const float4 *)(qr + 32 * j + 4);
-            }
-        }
-        const int pgs = shift - 5;                            // groups of a page, as a shift
+        const int pgs = c.shift - 5;                          // groups of a page, as a shift
         const int g_stop = few > 1 && wave >= few ? 0 : min(g_end, (hi + 31) >> 5);
         // the page and the byte of a group's keys and values; page -1: none
         auto locate = [&](int g, size_t *base) {
-            int page = table[(size_t)b * ld_table + (g >> pgs)];
-            if ((unsigned)page >= (unsigned)n_pages) page = -1;
-            *base = ((((size_t)max(page, 0) * a.n_kv + kvh) << shift) + (size_t)(g & ((1 << pgs) - 1)) * 32) * HD;
+            int page = table[(size_t)b * c.ld_table + (g >> pgs)];
+            if ((unsigned)page >= (unsigned)c.n_pages) page = -1;
+            *base = ((((size_t)max(page, 0) * a.n_kv + kvh) << c.shift) + (size_t)(g & ((1 << pgs) - 1)) * 32) * HD;
             return page;
         };
         uint4 kr[NJ], vr[NJ];
@@ -400,41 +322,22 @@ __global__ __launch_bounds__(AK_THREADS, NQ == 1 ? 3 : 2) void vx_attention_kvq_
             for (int j = 0; j < NJ; j++) vr[j] = *(const uint4 *)(vc + base + lane * 16 + 1024 * j);
         }
 
+        // the queries' parts: each wavefront stores some dims, or its own tile
+        float qs;
+        const float qf = x0.scale(&qs);
 #pragma unroll
-        for (int i = 0; i < NQ; i++) {
-            float amax = 0.0f;
-#pragma unroll
-            for (int j = 0; j < NJ; j++) {
-                amax = fmaxf(amax, fmaxf(fmaxf(fabsf(x0[i][j].x), fabsf(x0[i][j].y)), fmaxf(fabsf(x0[i][j].z), fabsf(x0[i][j].w))));
-                amax = fmaxf(amax, fmaxf(fmaxf(fabsf(x1[i][j].x), fabsf(x1[i][j].y)), fmaxf(fabsf(x1[i][j].z), fabsf(x1[i][j].w))));
-            }
-            amax = vx_max_x32(vx_max_x16(amax));
-            // below 2^14, so that the low parts stay normal numbers for long
-            float rs;
-            const float f = vx_row_scale(amax, &rs) * 16384.0f;
-            qs[i] *= rs;
-#pragma unroll
-            for (int j = 0; j < NJ; j++) {
-                if (few == 1 && (i * NJ + j) % AK_WAVES != wave) continue;
-                vx_half2 h[4], l[4];
-                vx_split(x0[i][j].x * f, x0[i][j].y * f, &h[0], &l[0]);
-                vx_split(x0[i][j].z * f, x0[i][j].w * f, &h[1], &l[1]);
-                vx_split(x1[i][j].x * f, x1[i][j].y * f, &h[2], &l[2]);
-                vx_split(x1[i][j].z * f, x1[i][j].w * f, &h[3], &l[3]);
-                sh.q[qw][i][0][j][lane] = *(const uint4 *)h;
-                sh.q[qw][i][1][j][lane] = *(const uint4 *)l;
-            }
+        for (int j = 0; j < NJ; j++) {
+            if (few == 1 && j % AK_WAVES != wave) continue;
+            vx_half2 h[4], l[4];
+            x0.parts(j, qf, h, l);
+            sh.q[qw][0][j][lane] = *(const uint4 *)h;
+            sh.q[qw][1][j][lane] = *(const uint4 *)l;
         }
         __syncthreads();
-        vx_f32x4 O[NQ][ND];
-        float m[NQ], l[NQ];
+        vx_f32x4 O[ND];
+        float m = -INFINITY, l = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NQ; i++) {
-            m[i] = -INFINITY;
-            l[i] = 0.0f;
-#pragma unroll
-            for (int d = 0; d < ND; d++) O[i][d] = vx_f32x4{};
-        }
+        for (int d = 0; d < ND; d++) O[d] = vx_f32x4{};
         for (; g < g_stop; g += stride) {
             // the next group's loads go out as this one's registers come free
             const bool more = g + stride < g_stop;
@@ -445,140 +348,91 @@ __global__ __launch_bounds__(AK_THREADS, NQ == 1 ? 3 : 2) void vx_attention_kvq_
             const bool none = page < 0;
             const float ksc = none ? 0.0f : ks[hp], vsc = none ? 0.0f : vs[hp];
             page = next;
-            vx_f32x4 S[NQ][2];
-            {
-                // the parts' sums meet at the end: the small ones round by themselves
-                vx_f32x4 L[NQ][2];
+            vx_f32x4 S[2], L[2];                              // of the high and of the low parts
 #pragma unroll
-                for (int j = 0; j < NJ; j++) {
-                    const vx_half8 k0 = vx_kvq_half8<TYPE>(kr[j].x, kr[j].y), k1 = vx_kvq_half8<TYPE>(kr[j].z, kr[j].w);
-                    kr[j] = *(const uint4 *)(kn + 1024 * j);
-#pragma unroll
-                    for (int i = 0; i < NQ; i++) {
-                        const vx_half8 qh = __builtin_bit_cast(vx_half8, sh.q[qw][i][0][j][lane]);
-                        const vx_half8 ql = __builtin_bit_cast(vx_half8, sh.q[qw][i][1][j][lane]);
-                        S[i][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qh, j ? S[i][0] : vx_f32x4{}, 0, 0, 0);
-                        S[i][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qh, j ? S[i][1] : vx_f32x4{}, 0, 0, 0);
-                        L[i][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, ql, j ? L[i][0] : vx_f32x4{}, 0, 0, 0);
-                        L[i][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, ql, j ? L[i][1] : vx_f32x4{}, 0, 0, 0);
-                        AK_KEEP(S[i][0], k0, qh);
-                        AK_KEEP(S[i][1], k1, qh);
-                        AK_KEEP(L[i][0], k0, ql);
-                        AK_KEEP(L[i][1], k1, ql);
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < NQ; i++) {
-                    S[i][0] += L[i][0];
-                    S[i][1] += L[i][1];
-                }
+            for (int j = 0; j < NJ; j++) {
+                const vx_half8 k0 = vx_kvq_half8<TYPE>(kr[j].x, kr[j].y), k1 = vx_kvq_half8<TYPE>(kr[j].z, kr[j].w);
+                kr[j] = *(const uint4 *)(kn + 1024 * j);
+                const vx_half8 qh = __builtin_bit_cast(vx_half8, sh.q[qw][0][j][lane]);
+                const vx_half8 ql = __builtin_bit_cast(vx_half8, sh.q[qw][1][j][lane]);
+                S[0] = vx_mfma(k0, qh, j ? S[0] : vx_f32x4{});
+                S[1] = vx_mfma(k1, qh, j ? S[1] : vx_f32x4{});
+                L[0] = vx_mfma(k0, ql, j ? L[0] : vx_f32x4{});
+                L[1] = vx_mfma(k1, ql, j ? L[1] : vx_f32x4{});
             }
+            S[0] += L[0];
+            S[1] += L[1];
             const int t0 = 32 * g + 4 * g4;
-            vx_half8 ph[NQ], pl[NQ];
+            if (32 * g + 32 > lo || none) vx_kvq_mask(S, t0, none ? 0 : lim);
+            const float cs = fmaxf(qs * ksc, 1e-37f);         // -inf must not meet a zero
+            const float nm = fmaxf(m, vx_max_x32(vx_max_x16(vx_max8(S))) * cs), ref = nm == -INFINITY ? 0.0f : nm;
+            if (__any(nm > m)) {
+                const float f = __builtin_amdgcn_exp2f(m - ref);
+                l *= f;
 #pragma unroll
-            for (int i = 0; i < NQ; i++) {
-                if (32 * g + 32 > lo || none) {
-#pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        if (none || t0 + (e >> 2) * 16 + (e & 3) >= lim[i]) S[i][e >> 2][e & 3] = -INFINITY;
-                }
-                // a scale of zero: -inf must not meet a zero
-                const float c = fmaxf(qs[i] * ksc, 1e-37f);
-                float cm = fmaxf(fmaxf(fmaxf(S[i][0][0], S[i][0][1]), fmaxf(S[i][0][2], S[i][0][3])),
-                                 fmaxf(fmaxf(S[i][1][0], S[i][1][1]), fmaxf(S[i][1][2], S[i][1][3])));
-                cm = vx_max_x32(vx_max_x16(cm)) * c;
-                const float nm = fmaxf(m[i], cm), ref = nm == -INFINITY ? 0.0f : nm;
-                if (__any(nm > m[i])) {
-                    const float f = __builtin_amdgcn_exp2f(m[i] - ref);
-                    l[i] *= f;
-#pragma unroll
-                    for (int d = 0; d < ND; d++) O[i][d] *= f;
-                    m[i] = nm;
-                }
-                // probabilities times 2^14: their low parts stay normal numbers
-                const float sub = 14.0f - ref;
-                float p[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    p[e] = __builtin_amdgcn_exp2f(fmaf(S[i][e >> 2][e & 3], c, sub));
-                    l[i] += p[e];
-                }
-                vx_half2 h[4], w[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) vx_split(p[2 * e], p[2 * e + 1], &h[e], &w[e]);
-                ph[i] = vx_half8{h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
-                pl[i] = vx_half8{w[0][0], w[0][1], w[1][0], w[1][1], w[2][0], w[2][1], w[3][0], w[3][1]};
+                for (int d = 0; d < ND; d++) O[d] *= f;
+                m = nm;
             }
+            // probabilities times 2^14: their low parts stay normal numbers
+            const float sub = 14.0f - ref;
+            vx_half2 h[4], w[4];
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(S[e >> 2][e & 3], cs, sub));
+                const float p1 = __builtin_amdgcn_exp2f(fmaf(S[e >> 2][(e & 3) + 1], cs, sub));
+                l += p0 + p1;
+                vx_split(p0, p1, &h[e / 2], &w[e / 2]);
+            }
+            const vx_half8 ph = vx_join8(h), pl = vx_join8(w);
             if (TYPE == VXH_KVQ_E4M3 && (none || 32 * g + 32 > hi)) {
-                // codes that no query reads may be NaN, and 0 times it is
-                uint32_t mk[2] = {0, 0};
 #pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (!none && t0 + (e >> 2) * 16 + (e & 3) < hi) mk[e >> 2] |= 0xFFu << (8 * (e & 3));
-#pragma unroll
-                for (int j = 0; j < NJ; j++)
-                    vr[j] = make_uint4(vr[j].x & mk[0], vr[j].y & mk[1], vr[j].z & mk[0], vr[j].w & mk[1]);
+                for (int j = 0; j < NJ; j++) vr[j] = vx_kvq_mask_codes(vr[j], t0, none ? 0 : hi);
             }
 #pragma unroll
             for (int j = 0; j < NJ; j++) {
                 const vx_half8 v0 = vx_kvq_half8<TYPE>(vr[j].x, vr[j].y), v1 = vx_kvq_half8<TYPE>(vr[j].z, vr[j].w);
                 vr[j] = *(const uint4 *)(vn + 1024 * j);
+                vx_f32x4 t = vx_mfma(v0, pl, vx_f32x4{}), u = vx_mfma(v1, pl, vx_f32x4{});
+                t = vx_mfma(v0, ph, t);
+                u = vx_mfma(v1, ph, u);
 #pragma unroll
-                for (int i = 0; i < NQ; i++) {
-                    vx_f32x4 t = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl[i], vx_f32x4{}, 0, 0, 0);
-                    vx_f32x4 u = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl[i], vx_f32x4{}, 0, 0, 0);
-                    AK_KEEP(t, v0, pl[i]);
-                    AK_KEEP(u, v1, pl[i]);
-                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph[i], t, 0, 0, 0);
-                    u = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph[i], u, 0, 0, 0);
-                    AK_KEEP(t, v0, ph[i]);
-                    AK_KEEP(u, v1, ph[i]);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        O[i][2 * j][e] = fmaf(t[e], vsc, O[i][2 * j][e]);
-                        O[i][2 * j + 1][e] = fmaf(u[e], vsc, O[i][2 * j + 1][e]);
-                    }
+                for (int e = 0; e < 4; e++) {
+                    O[2 * j][e] = fmaf(t[e], vsc, O[2 * j][e]);
+                    O[2 * j + 1][e] = fmaf(u[e], vsc, O[2 * j + 1][e]);
                 }
             }
         }
 
         auto finish = [&](int qi, int d, vx_f32x4 o, float sum) {
             const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
-            *(vx_f32x4 *)(out + (size_t)(s.row + qi / a.G) * ld_out + (size_t)(kvh * a.G + qi % a.G) * HD + d) = o * inv;
+            *(vx_f32x4 *)(out + (size_t)(s.row + qi / a.G) * c.ld_out + (size_t)(kvh * a.G + qi % a.G) * HD + d) = o * inv;
         };
-#pragma unroll
-        for (int i = 0; i < NQ; i++) l[i] = vx_sum_x32(vx_sum_x16(l[i]));
+        l = vx_sum_x32(vx_sum_x16(l));
         if (few > 1) {
+            if (wave < few && ok)
 #pragma unroll
-            for (int i = 0; i < NQ; i++)
-                if (wave < few && q0 + 16 * i + n < s.nq)
-#pragma unroll
-                    for (int d = 0; d < ND; d++) finish(q0 + 16 * i + n, 16 * d + 4 * g4, O[i][d], l[i]);
+                for (int d = 0; d < ND; d++) finish(qi, 16 * d + 4 * g4, O[d], l);
             x = first + (int64_t)few * (groups + AK_BEGIN);
             __syncthreads();
             if (x < w_end) {
-                vx_kvq_find<QT>(a, list, x, 0);
+                vx_kvq_find(a, list, x, 0);
                 __syncthreads();
             }
             continue;
         }
         // the wavefronts' parts meet in LDS
         __syncthreads();
+        {
+            float *so = sh.o[wave][n];
 #pragma unroll
-        for (int i = 0; i < NQ; i++) {
-            float *so = sh.o[wave][16 * i + n];
-#pragma unroll
-            for (int d = 0; d < ND; d++) *(vx_f32x4 *)(so + 16 * d + 4 * g4) = O[i][d];
-            if (g4 == 0) {
-                so[HD] = m[i];
-                so[HD + 1] = l[i];
-            }
+            for (int d = 0; d < ND; d++) *(vx_f32x4 *)(so + 16 * d + 4 * g4) = O[d];
+            if (g4 == 0) *(float2 *)(so + HD) = make_float2(m, l);
         }
         __syncthreads();
         const bool whole = g_begin == 0 && g_end == groups;
         // a piece holds at most one tile begun before it and one that goes on behind it
-        float *mine_p = part + (size_t)(2 * blockIdx.x + (g_begin == 0)) * QT * PS;
-        const int nv = min(QT, s.nq - q0);
+        float *mine_p = part + (size_t)(2 * blockIdx.x + (g_begin == 0)) * 16 * PS;
+        const int nv = min(16, s.nq - q0);
         for (int u = tid; u < nv * (HD / 4); u += AK_THREADS) {
             const int qq = u / (HD / 4), d = u % (HD / 4) * 4;
             float mx = sh.o[0][qq][HD];
@@ -621,8 +475,8 @@ __global__ __launch_bounds__(AK_THREADS, NQ == 1 ? 3 : 2) void vx_attention_kvq_
             bool last = c1 - c0 == 1 || vx_arrive(counter + p0 + blk, c1 - c0, &s_last);
             if (last && n_blk > 1) {
                 if (c1 - c0 > 1)
-                    vx_kvq_join<HD, QT, AK_THREADS>(part, slot0, c0, c1, nv, [&](int qq, int d, vx_f32x4 o, float mx, float sum) {
-                        float *pp = part + ((size_t)slot1(blk) * QT + qq) * PS;
+                    vx_kvq_join<HD>(part, slot0, c0, c1, nv, [&](int qq, int d, vx_f32x4 o, float mx, float sum) {
+                        float *pp = part + ((size_t)slot1(blk) * 16 + qq) * PS;
                         vx_dev_store2(pp + d, o[0], o[1]);
                         vx_dev_store2(pp + d + 2, o[2], o[3]);
                         if (d == 0) vx_dev_store2(pp + HD, mx, sum);
@@ -630,13 +484,13 @@ __global__ __launch_bounds__(AK_THREADS, NQ == 1 ? 3 : 2) void vx_attention_kvq_
                 last = vx_arrive(counter + AK_WG + p0, n_blk, &s_last);
             }
             auto put = [&](int qq, int d, vx_f32x4 o, float mx, float sum) { finish(q0 + qq, d, o, sum); };
-            if (last && n_blk > 1) vx_kvq_join<HD, QT, AK_THREADS>(part, slot1, 0, n_blk, nv, put);
-            else if (last) vx_kvq_join<HD, QT, AK_THREADS>(part, slot0, 0, c1, nv, put);
+            if (last && n_blk > 1) vx_kvq_join<HD>(part, slot1, 0, n_blk, nv, put);
+            else if (last) vx_kvq_join<HD>(part, slot0, 0, c1, nv, put);
         }
         x = first + AK_BEGIN + g_end;
         if (x < w_end) {
             __syncthreads();
-            vx_kvq_find<QT>(a, list, x, 0);
+            vx_kvq_find(a, list, x, 0);
             __syncthreads();
         }
     }
@@ -645,6 +499,8 @@ __global__ __launch_bounds__(AK_THREADS, NQ == 1 ? 3 : 2) void vx_attention_kvq_
 extern "C" size_t vxh_attention_kvq_workspace_floats(int max_rows, int n_seqs, int n_heads, int n_kv_heads,
                                                      int head_dim)
 {
+    // two parts a piece, whatever the batch
+    (void)max_rows, (void)n_seqs, (void)n_heads, (void)n_kv_heads;
     return (size_t)2 * AK_WG * 16 * (head_dim + 4);
 }
 
@@ -661,28 +517,45 @@ extern "C" int vxh_attention_kvq(const float *q, int ldq, const int *row0, const
         ws->part_floats < vxh_attention_kvq_workspace_floats(max_rows, n_seqs, n_heads, c->n_kv_heads, c->head_dim))
         return vxh_fail(VXH_ERR_PARAM, "attention_kvq: %d requests, %d rows, %d/%d heads of %d (ld %d, %d)", n_seqs,
                         max_rows, n_heads, c->n_kv_heads, c->head_dim, ldq, ld_out);
-    vx_kvq_batch a;
-    a.row0 = row0;
-    a.len = len;
-    a.B = n_seqs;
-    a.max_rows = max_rows;
-    a.n_kv = c->n_kv_heads;
-    a.G = n_heads / c->n_kv_heads;
-    a.cap = cap;
     const int64_t limit = (int64_t)ld_table * c->page;
-    a.limit = limit > 0x7FFFFF00 ? 0x7FFFFF00 : (int)limit;
-    const int shift = c->page == 32 ? 5 : c->page == 64 ? 6 : 7;
+    vx_kvq_call call;
+    call.a.row0 = row0;
+    call.a.len = len;
+    call.a.B = n_seqs;
+    call.a.max_rows = max_rows;
+    call.a.n_kv = c->n_kv_heads;
+    call.a.G = n_heads / c->n_kv_heads;
+    call.a.cap = cap;
+    call.a.limit = limit > 0x7FFFFF00 ? 0x7FFFFF00 : (int)limit;
+    call.a.few = 0x7FFFFFFF;
+    call.q = q;
+    call.ldq = ldq;
+    call.table = table;
+    call.ld_table = ld_table;
+    call.kc = (const uint8_t *)c->k;
+    call.vc = (const uint8_t *)c->v;
+    call.ks = c->ks;
+    call.vs = c->vs;
+    call.shift = c->page == 32 ? 5 : c->page == 64 ? 6 : 7;
+    call.n_pages = c->n_pages;
+    call.out = out;
+    call.ld_out = ld_out;
+    call.part = ws->part;
+    if (vx_kvq_many_wanted(call.a, max_seq_rows)) {
+        // of one request the host knows the rows: nothing is left for the other kernel
+        call.a.few = n_seqs == 1 ? 0 : AK_FEW;
+        int rc = vx_kvq_many(call, c->type, c->head_dim, vxh_hs(s));
+        if (rc || n_seqs == 1) return rc;
+    }
     unsigned *counter = (unsigned *)(ws->acc + ws->acc_elems);
-#define VX_CALL(T, HD, NQ)                                                                                            \
-    vx_attention_kvq_kernel<T, HD, NQ><<<AK_WG, AK_THREADS, 0, vxh_hs(s)>>>(                                           \
-        q, ldq, a, table, ld_table, (const uint8_t *)c->k, (const uint8_t *)c->v, c->ks, c->vs, shift, c->n_pages,    \
-        out, ld_out, ws->part, counter)
+#define VX_CALL(T, HD) vx_attention_kvq_kernel<T, HD><<<AK_WG, AK_THREADS, 0, vxh_hs(s)>>>( \
+        call, call.q, call.table, call.kc, call.vc, call.ks, call.vs, call.out, call.part, counter)
 #define VX_HD(T)                                                                                                      \
     switch (c->head_dim) {                                                                                            \
-    case 32: VX_CALL(T, 32, 1); break;                                                                                     \
-    case 64: VX_CALL(T, 64, 1); break;                                                                                     \
-    case 96: VX_CALL(T, 96, 1); break;                                                                                     \
-    default: VX_CALL(T, 128, 1);                                                                                           \
+    case 32: VX_CALL(T, 32); break;                                                                                   \
+    case 64: VX_CALL(T, 64); break;                                                                                   \
+    case 96: VX_CALL(T, 96); break;                                                                                   \
+    default: VX_CALL(T, 128);                                                                                         \
     }
     if (c->type == VXH_KVQ_INT8) {
         VX_HD(VXH_KVQ_INT8)
