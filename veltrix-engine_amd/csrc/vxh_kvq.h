@@ -64,6 +64,24 @@ __device__ __forceinline__ uint32_t vx_kvq_code(float x, float s, float inv)
     return x != x ? 0u : (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, 0.0f, 0, false) & 0xFFu;
 }
 
+// The same from a product with inv for finite x of |x| <= top s: the low byte,
+// and *sure false where that product lies so near a border between two codes
+// (or so near zero, e4m3) that only vx_kvq_code can tell.
+template <int TYPE>
+__device__ __forceinline__ uint32_t vx_kvq_code_fast(float x, float s, float inv, bool *sure)
+{
+    const float y = x * inv;
+    if (TYPE == VXH_KVQ_INT8) {
+        const float t = rintf(y);
+        *sure &= fabsf(y - t) < 0.4999f;
+        return (uint32_t)((int)t + 128);
+    }
+    // an e4m3 code has 3 of 23 mantissa bits: a border is a half of the other 20
+    const int b = __float_as_int(y);
+    *sure &= fabsf(y) >= 0x1p-6f && abs((b & 0xFFFFF) - 0x80000) > 4;
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, 0.0f, 0, false) & 0xFFu;
+}
+
 // Code of a stored code's value v (at the scale s0 <= s) at the scale s.
 template <int TYPE>
 __device__ __forceinline__ uint32_t vx_kvq_recode(float v, float s0, float s)

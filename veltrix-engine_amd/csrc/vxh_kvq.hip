@@ -189,152 +189,162 @@ extern "C" int vxh_page_tables(const int *len, const int *add, int n_seqs, int p
 }
 
 // ---------------------------------------------------------------------------
-// Write.  A workgroup owns one (page, kv head) of K or of V: a page's first
-// row in the batch names it, and every other row of the page, wherever it
+// Write.  A workgroup owns pages of K or V of some heads: the first of the
+// batch's rows on a page names it, and every other row of the page, wherever it
 // stands, is found by one pass over the slots.  So a scale has one writer and
 // the result does not depend on the order of workgroups.  The rows are read
-// once, into registers; their codes meet in LDS and leave as whole 16-byte
-// lanes of the cache's layout.
+// once, into registers; their codes meet in LDS in the cache's order and leave
+// as whole 16-byte lanes, blended with the page's other tokens.
 // ---------------------------------------------------------------------------
 #define KW_THREADS 256
+#define KW_PIECES 256            // of the rows
+#define KW_WG 2048               // workgroups; heads past that in turn
 
-template <int TYPE>
+// Bytes of a word whose bits 0..3 are set in nib.
+__device__ __forceinline__ uint32_t vx_spread(uint32_t nib) { return (((nib & 15u) * 0x00204081u) & 0x01010101u) * 0xFFu; }
+
+template <int TYPE, int PG>
 __global__ __launch_bounds__(KW_THREADS) void vx_kvq_write_kernel(vxh_kvq c, const float *__restrict__ k, int ldk,
                                                                   const float *__restrict__ v, int ldv,
-                                                                  const int *__restrict__ slot, int R)
+                                                                  const int *__restrict__ slot, int R, int chunk)
 {
-    __shared__ int s_src[KVQ_MAX_PAGE], s_first, s_count[KW_THREADS / 64], s_lead;
+    constexpr int P = 32 * PG, SHIFT = PG == 1 ? 5 : PG == 2 ? 6 : 7, NI = 4 * PG;
+    __shared__ int s_src[P], s_first;
+    __shared__ uint32_t s_has[PG];                       // the page's tokens that come, a bit each
     __shared__ float s_amax[KW_THREADS / 64];
-    __shared__ __align__(16) uint8_t s_code[KVQ_MAX_PAGE * (128 + 16)];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int P = c.page, hd = c.head_dim, head = blockIdx.y, ldc = hd + 16;
-    const bool is_v = blockIdx.z;
-    const float *x = is_v ? v : k;
-    const int ldx = is_v ? ldv : ldk;
-    uint8_t *cache = (uint8_t *)(is_v ? c.v : c.k);
-    float *scales = is_v ? c.vs : c.ks;
-    auto page_of = [&](int r) {
-        const int sl = slot[r];
-        return sl < 0 || sl / P >= c.n_pages ? -1 : sl / P;
-    };
-    // candidates: rows whose predecessor lies on another page, counted in order
-    const int E = (R + KW_THREADS - 1) / KW_THREADS, r0 = min(tid * E, R), r1 = min(r0 + E, R);
-    int mine = 0;
-    {
-        int before = r0 > 0 && r0 < R ? page_of(r0 - 1) : -1;
-        for (int r = r0; r < r1; r++) {
-            const int p = page_of(r);
-            mine += p >= 0 && p != before;
-            before = p;
-        }
-    }
-    int at = mine;
-    for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(at, o);
-        if (lane >= o) at += u;
-    }
-    if (lane == 63) s_count[wave] = at;
-    __syncthreads();
-    int total = 0;
-    at -= mine;
-    for (int w = 0; w < KW_THREADS / 64; w++) {
-        if (w < wave) at += s_count[w];
-        total += s_count[w];
-    }
-    for (int cand = blockIdx.x; cand < total; cand += gridDim.x) {
+    __shared__ uint4 s_code[P * 128 / 16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hd = c.head_dim;
+    const unsigned n_pages = c.n_pages;
+    const int n4 = hd / 4;                               // items of 4 dims a token
+    const float per4 = 1.0f / n4;
+    auto token = [&](int it) { return (int)(((float)it + 0.5f) * per4); };
+    auto page_of = [&](int sl) { return sl < 0 || (unsigned)(sl >> SHIFT) >= n_pages ? -1 : sl >> SHIFT; };
+    const int r1 = min((int)(blockIdx.y + 1) * chunk, R);
+    for (int lead = blockIdx.y * chunk; lead < r1; lead++) {
+        // rows behind another of their page are that one's
+        const int page = page_of(slot[lead]);
+        if (page < 0 || (lead > 0 && page_of(slot[lead - 1]) == page)) continue;
         __syncthreads();
-        if (cand >= at && cand < at + mine) {            // the thread that counted it finds its row
-            int i = at, before = r0 > 0 ? page_of(r0 - 1) : -1;
-            for (int r = r0; r < r1; r++) {
-                const int p = page_of(r);
-                if (p >= 0 && p != before && i++ == cand) {
-                    s_lead = r;
-                    break;
-                }
-                before = p;
-            }
-        }
         if (tid == 0) s_first = R;
         for (int i = tid; i < P; i += KW_THREADS) s_src[i] = -1;
+        if (tid < PG) s_has[tid] = 0;
         __syncthreads();
-        const int lead = s_lead, page = page_of(lead);
-        for (int r = tid; r < R; r += KW_THREADS)
-            if (page_of(r) == page) {
-                atomicMin(&s_first, r);
-                atomicMax(&s_src[slot[r] % P], r);       // the same slot twice: the later row
-            }
+        for (int r0 = tid; r0 < R; r0 += 8 * KW_THREADS) {
+            int sl[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) sl[i] = r0 + i * KW_THREADS < R ? slot[r0 + i * KW_THREADS] : -1;
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (page_of(sl[i]) == page) {
+                    const int r = r0 + i * KW_THREADS, t = sl[i] & (P - 1);
+                    atomicMin(&s_first, r);
+                    atomicMax(&s_src[t], r);             // the same slot twice: the later row
+                    atomicOr(&s_has[t >> 5], 1u << (t & 31));
+                }
+        }
         __syncthreads();
-        if (s_first != lead) continue;                   // an earlier candidate has this page
+        if (s_first != lead) continue;                   // an earlier row has this page
 
-        const size_t base = ((size_t)page * c.n_kv_heads + head) * (size_t)(P * hd);
-        float *sp = scales + (size_t)page * c.n_kv_heads + head;
-        const int n4 = hd / 4, items = P * n4;           // 16 items a thread at most
-        float4 val[KVQ_MAX_PAGE * 128 / 4 / KW_THREADS];
-        float amax = 0.0f;
+        // a part's rows, this thread's items of 4 dims; the next part's are on
+        // their way while one is worked on
+        float4 val[NI];
+        auto fetch = [&](int part) {
+            const bool is_v = part >= c.n_kv_heads;
+            const int ldx = is_v ? ldv : ldk;
+            const float *x = is_v ? v + (part - c.n_kv_heads) * hd : k + part * hd;
 #pragma unroll
-        for (int i = 0; i < KVQ_MAX_PAGE * 128 / 4 / KW_THREADS; i++) {
-            const int it = tid + i * KW_THREADS;
-            val[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (it < items) {
-                const int src = s_src[it / n4];
-                if (src >= 0) val[i] = *(const float4 *)(x + (size_t)src * ldx + head * hd + 4 * (it % n4));
+            for (int i = 0; i < NI; i++) {
+                const int it = tid + i * KW_THREADS, t = token(it);
+                const int src = t < P ? s_src[t] : -1;
+                val[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (src >= 0) val[i] = *(const float4 *)(x + (size_t)src * ldx + 4 * (it - t * n4));
             }
-            const float a[4] = {val[i].x, val[i].y, val[i].z, val[i].w};
+        };
+        fetch(blockIdx.x);
+        for (int part = blockIdx.x; part < 2 * c.n_kv_heads; part += gridDim.x) {
+            const bool is_v = part >= c.n_kv_heads;
+            const int head = is_v ? part - c.n_kv_heads : part;
+            const size_t hp = (size_t)page * c.n_kv_heads + head;
+            uint4 *dst = (uint4 *)((uint8_t *)(is_v ? c.v : c.k) + hp * (size_t)(P * hd));
+            float *sp = (is_v ? c.vs : c.ks) + hp;
+            const float held = *sp;
+            float amax = 0.0f;
+            bool finite = true;
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (fabsf(a[e]) < INFINITY) amax = fmaxf(amax, fabsf(a[e]));
-        }
-        amax = vx_wave_max64(amax);
-        if (lane == 0) s_amax[wave] = amax;
-        __syncthreads();
-        for (int w = 0; w < KW_THREADS / 64; w++) amax = fmaxf(amax, s_amax[w]);
-        const float fit = amax >= 0x1p-100f ? amax / (TYPE == VXH_KVQ_INT8 ? 127.0f : 448.0f) : 0.0f;
-        const bool start = s_src[0] >= 0;
-        const float s_old = start ? 0.0f : *sp;
-        const float sc = fmaxf(s_old, fit), inv = sc > 0.0f ? 1.0f / sc : 0.0f;
-        const bool grown = sc > s_old && !start;
-#pragma unroll
-        for (int i = 0; i < KVQ_MAX_PAGE * 128 / 4 / KW_THREADS; i++) {
-            const int it = tid + i * KW_THREADS;
-            if (it < items && s_src[it / n4] >= 0) {
+            for (int i = 0; i < NI; i++) {
                 const float a[4] = {val[i].x, val[i].y, val[i].z, val[i].w};
-                uint32_t w = 0;
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    w |= (sc > 0.0f ? vx_kvq_code<TYPE>(a[e], sc, inv) : TYPE == VXH_KVQ_INT8 ? 128u : 0u) << (8 * e);
-                *(uint32_t *)(s_code + (it / n4) * ldc + 4 * (it % n4)) = w;
+                for (int e = 0; e < 4; e++) {
+                    const bool f = fabsf(a[e]) < INFINITY;
+                    finite &= f;
+                    amax = fmaxf(amax, f ? fabsf(a[e]) : 0.0f);
+                }
             }
-        }
-        __syncthreads();
-        if (tid == 0) *sp = sc;
-        // lanes of 16 codes: K holds 8 dims of two tokens, V 8 tokens of two dims
-        for (int u = tid; u < P * hd / 16; u += KW_THREADS) {
-            const int ln = u & 63, g = ln >> 4, n = ln & 15, grp = u >> 6;
-            const int t0 = grp / (hd / 32) * 32, d0 = grp % (hd / 32) * 32;
-            uint8_t *dst = cache + base + (size_t)u * 16;
-            int tok[16], dim[16];
-            bool any = false, all = true;
+            amax = vx_wave_max64(amax);
+            if (lane == 0) s_amax[wave] = amax;
+            __syncthreads();
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                tok[e] = is_v ? t0 + ((e >> 2) & 1) * 16 + 4 * g + (e & 3) : t0 + (e >> 3) * 16 + n;
-                dim[e] = is_v ? d0 + (e >> 3) * 16 + n : d0 + 8 * g + (e & 7);
-                const bool in = s_src[tok[e]] >= 0;
-                any |= in;
-                all &= in;
-            }
-            if (!any && !grown) continue;
-            uint4 old = make_uint4(0, 0, 0, 0);
-            if (!all) old = *(const uint4 *)dst;
-            uint32_t w[4] = {old.x, old.y, old.z, old.w};
+            for (int w = 0; w < KW_THREADS / 64; w++) amax = fmaxf(amax, s_amax[w]);
+            const float fit = amax >= 0x1p-100f ? amax / (TYPE == VXH_KVQ_INT8 ? 127.0f : 448.0f) : 0.0f;
+            const bool start = s_has[0] & 1;             // the page's first token starts it anew
+            const float s_old = start ? 0.0f : held, sc = fmaxf(s_old, fit), inv = sc > 0.0f ? 1.0f / sc : 0.0f;
+            const bool grown = sc > s_old && !start;
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const int sh = 8 * (e & 3);
-                uint32_t code = (w[e >> 2] >> sh) & 0xFFu;
-                if (s_src[tok[e]] >= 0) code = s_code[tok[e] * ldc + dim[e]];
-                else if (grown) code = vx_kvq_recode<TYPE>(vx_kvq_value<TYPE>(code), s_old, sc);
-                w[e >> 2] = (w[e >> 2] & ~(0xFFu << sh)) | (code << sh);
+            for (int i = 0; i < NI; i++) {
+                const int it = tid + i * KW_THREADS, t = token(it), d = 4 * (it - t * n4);
+                if (t < P && s_src[t] >= 0) {
+                    const float a[4] = {val[i].x, val[i].y, val[i].z, val[i].w};
+                    uint32_t code[4];
+                    bool sure = finite && sc > 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) code[e] = vx_kvq_code_fast<TYPE>(a[e], sc, inv, &sure);
+                    if (!sure) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            code[e] = sc > 0.0f ? vx_kvq_code<TYPE>(a[e], sc, inv) : TYPE == VXH_KVQ_INT8 ? 128u : 0u;
+                    }
+                    if (is_v) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) ((uint8_t *)s_code)[vx_kvq_v_byte(t, d + e, hd)] = (uint8_t)code[e];
+                    } else
+                        *(uint32_t *)((uint8_t *)s_code + vx_kvq_k_byte(t, d, hd)) =
+                            code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24;
+                }
             }
-            *(uint4 *)dst = make_uint4(w[0], w[1], w[2], w[3]);
+            if (part + (int)gridDim.x < 2 * c.n_kv_heads) fetch(part + gridDim.x);
+            __syncthreads();
+            if (tid == 0) *sp = sc;
+            // lanes of 16 codes: K holds 8 dims of two tokens, V 8 tokens of two dims
+            for (int u = tid; u < P * hd / 16; u += KW_THREADS) {
+                const uint32_t has = s_has[(u >> 6) / (hd / 32)];
+                const int g = (u >> 4) & 3, n = u & 15;
+                uint32_t m0, m1, m2, m3;
+                if (is_v) {
+                    m0 = m2 = vx_spread(has >> (4 * g));
+                    m1 = m3 = vx_spread(has >> (16 + 4 * g));
+                } else {
+                    m0 = m1 = has >> n & 1 ? ~0u : 0u;
+                    m2 = m3 = has >> (n + 16) & 1 ? ~0u : 0u;
+                }
+                if (!(m0 | m1 | m2) && !grown) continue;
+                uint4 w = s_code[u];
+                if ((m0 & m1 & m2) != ~0u) {
+                    uint4 old = dst[u];
+                    if (grown) {
+                        uint32_t o[4] = {old.x, old.y, old.z, old.w};
+#pragma unroll
+                        for (int e = 0; e < 16; e++) {
+                            const int sh = 8 * (e & 3);
+                            const uint32_t code = vx_kvq_recode<TYPE>(vx_kvq_value<TYPE>((o[e >> 2] >> sh) & 0xFFu), s_old, sc);
+                            o[e >> 2] = (o[e >> 2] & ~(0xFFu << sh)) | (code << sh);
+                        }
+                        old = make_uint4(o[0], o[1], o[2], o[3]);
+                    }
+                    w = make_uint4((w.x & m0) | (old.x & ~m0), (w.y & m1) | (old.y & ~m1), (w.z & m2) | (old.z & ~m2),
+                                   (w.w & m3) | (old.w & ~m3));
+                }
+                dst[u] = w;
+            }
         }
     }
 }
@@ -355,37 +365,80 @@ extern "C" int vxh_kvq_write(const vxh_kvq *c, const float *k, int ldk, const fl
 {
     int rc = vx_kvq_rows_check("kvq_write", c, k, ldk, v, ldv, slot, R);
     if (rc) return rc;
-    int gx = 4096 / (2 * c->n_kv_heads);
-    gx = gx < 1 ? 1 : gx > R ? R : gx;
-    const dim3 grid(gx, c->n_kv_heads, 2);
-    if (c->type == VXH_KVQ_INT8)
-        vx_kvq_write_kernel<VXH_KVQ_INT8><<<grid, KW_THREADS, 0, vxh_hs(s)>>>(*c, k, ldk, v, ldv, slot, R);
-    else
-        vx_kvq_write_kernel<VXH_KVQ_E4M3><<<grid, KW_THREADS, 0, vxh_hs(s)>>>(*c, k, ldk, v, ldv, slot, R);
+    // A prompt's pages begin every 32nd row or so: an odd piece length keeps the
+    // workgroups that find one off one XCD (2048 rows, 32 heads of 128: 153 us
+    // with all on one, 37 spread; 512 pieces with 8192 workgroups 41).
+    const int chunk = R <= KW_PIECES ? 1 : (R + KW_PIECES - 1) / KW_PIECES | 1, gy = (R + chunk - 1) / chunk;
+    int gx = 2 * c->n_kv_heads;
+    if (gx > KW_WG / gy) gx = KW_WG / gy;
+    const dim3 grid(gx, gy);
+#define VX_CALL(T, PG) vx_kvq_write_kernel<T, PG><<<grid, KW_THREADS, 0, vxh_hs(s)>>>(*c, k, ldk, v, ldv, slot, R, chunk)
+#define VX_PAGE(T)                                                                                                    \
+    if (c->page == 32) VX_CALL(T, 1);                                                                                 \
+    else if (c->page == 64) VX_CALL(T, 2);                                                                            \
+    else VX_CALL(T, 4);
+    if (c->type == VXH_KVQ_INT8) {
+        VX_PAGE(VXH_KVQ_INT8)
+    } else {
+        VX_PAGE(VXH_KVQ_E4M3)
+    }
+#undef VX_PAGE
+#undef VX_CALL
     VXH_LAUNCHED();
     return VXH_OK;
 }
 
 // ---------------------------------------------------------------------------
-// Read-back: one thread per 8 dims of a row's K and V head.
+// Read-back.  A workgroup takes 32 rows of one kv head's K or V.  Rows that are
+// 32 tokens of a page in order (a request read from its start) come as whole
+// lanes of the cache through LDS; any others code by code.
 // ---------------------------------------------------------------------------
 template <int TYPE>
 __global__ __launch_bounds__(256) void vx_kvq_read_kernel(vxh_kvq c, const int *__restrict__ slot, int R,
-                                                          float *__restrict__ k, int ldk, float *__restrict__ v, int ldv)
+                                                          float *__restrict__ k, int ldk, float *__restrict__ v, int ldv,
+                                                          int shift)
 {
-    const int hd = c.head_dim, per_row = c.n_kv_heads * hd / 8;
-    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    const int r = (int)(i / per_row), u = (int)(i % per_row), head = u / (hd / 8), d = u % (hd / 8) * 8;
-    if (r >= R) return;
-    const int sl = slot[r], page = sl / c.page, t = sl % c.page;
-    if (sl < 0 || page >= c.n_pages) return;
-    const size_t hp = (size_t)page * c.n_kv_heads + head, base = hp * (size_t)(c.page * hd);
-    const float ks = c.ks[hp], vs = c.vs[hp];
-    const uint8_t *kp = (const uint8_t *)c.k + base, *vp = (const uint8_t *)c.v + base;
+    __shared__ float s_row[32][128 + 4];
+    const int tid = threadIdx.x, hd = c.head_dim, n4 = hd / 4, r0 = blockIdx.y * 32;
+    const bool is_v = (int)blockIdx.x >= c.n_kv_heads;
+    const int head = is_v ? blockIdx.x - c.n_kv_heads : blockIdx.x, ldx = is_v ? ldv : ldk;
+    float *x = (is_v ? v : k) + head * hd;
+    const uint8_t *codes = (const uint8_t *)(is_v ? c.v : c.k);
+    const float *scales = is_v ? c.vs : c.ks;
+    const int s0 = slot[r0], mine = r0 + (tid & 31) < R ? slot[r0 + (tid & 31)] : -1;
+    const bool whole = __all(mine == s0 + (tid & 31)) && s0 >= 0 && s0 % 32 == 0 && (s0 >> shift) < c.n_pages;
+    if (whole) {                                         // (the same in every wavefront)
+        const size_t hp = (size_t)(s0 >> shift) * c.n_kv_heads + head;
+        const float sc = scales[hp];
+        const uint4 *src = (const uint4 *)(codes + (hp << shift) * hd + (size_t)(s0 & ((1 << shift) - 1)) * hd);
+        for (int u = tid; u < 2 * hd; u += 256) {        // 64 lanes for each 32 dims
+            const uint4 w = src[u];
+            const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+            const int g = (u >> 4) & 3, n = u & 15, d0 = u / 64 * 32;
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        k[(size_t)r * ldk + head * hd + d + e] = vx_kvq_value<TYPE>(kp[vx_kvq_k_byte(t, d + e, hd)]) * ks;
-        v[(size_t)r * ldv + head * hd + d + e] = vx_kvq_value<TYPE>(vp[vx_kvq_v_byte(t, d + e, hd)]) * vs;
+            for (int e = 0; e < 16; e++) {
+                const float f = vx_kvq_value<TYPE>((word[e >> 2] >> (8 * (e & 3))) & 0xFFu) * sc;
+                if (is_v) s_row[((e >> 2) & 1) * 16 + 4 * g + (e & 3)][d0 + (e >> 3) * 16 + n] = f;
+                else s_row[(e >> 3) * 16 + n][d0 + 8 * g + (e & 7)] = f;
+            }
+        }
+        __syncthreads();
+        for (int i = tid; i < 32 * n4; i += 256)
+            *(float4 *)(x + (size_t)(r0 + i / n4) * ldx + 4 * (i % n4)) = *(const float4 *)&s_row[i / n4][4 * (i % n4)];
+        return;
+    }
+    for (int i = tid; i < 32 * n4; i += 256) {
+        const int r = r0 + i / n4, d = 4 * (i % n4), sl = r < R ? slot[r] : -1;
+        if (sl < 0 || (sl >> shift) >= c.n_pages) continue;
+        const int t = sl & ((1 << shift) - 1);
+        const size_t hp = (size_t)(sl >> shift) * c.n_kv_heads + head;
+        const uint8_t *p = codes + (hp << shift) * hd;
+        const float sc = scales[hp];
+        float f[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            f[e] = vx_kvq_value<TYPE>(p[is_v ? vx_kvq_v_byte(t, d + e, hd) : vx_kvq_k_byte(t, d + e, hd)]) * sc;
+        *(float4 *)(x + (size_t)r * ldx + d) = make_float4(f[0], f[1], f[2], f[3]);
     }
 }
 
@@ -394,12 +447,12 @@ extern "C" int vxh_kvq_read(const vxh_kvq *c, const int *slot, int R, float *k, 
 {
     int rc = vx_kvq_rows_check("kvq_read", c, k, ldk, v, ldv, slot, R);
     if (rc) return rc;
-    const int64_t n = (int64_t)R * c->n_kv_heads * c->head_dim / 8;
-    const unsigned grid = (unsigned)((n + 255) / 256);
+    const int shift = c->page == 32 ? 5 : c->page == 64 ? 6 : 7;
+    const dim3 grid(2 * c->n_kv_heads, (R + 31) / 32);
     if (c->type == VXH_KVQ_INT8)
-        vx_kvq_read_kernel<VXH_KVQ_INT8><<<grid, 256, 0, vxh_hs(s)>>>(*c, slot, R, k, ldk, v, ldv);
+        vx_kvq_read_kernel<VXH_KVQ_INT8><<<grid, 256, 0, vxh_hs(s)>>>(*c, slot, R, k, ldk, v, ldv, shift);
     else
-        vx_kvq_read_kernel<VXH_KVQ_E4M3><<<grid, 256, 0, vxh_hs(s)>>>(*c, slot, R, k, ldk, v, ldv);
+        vx_kvq_read_kernel<VXH_KVQ_E4M3><<<grid, 256, 0, vxh_hs(s)>>>(*c, slot, R, k, ldk, v, ldv, shift);
     VXH_LAUNCHED();
     return VXH_OK;
 }
