@@ -74,6 +74,19 @@ typedef struct {
 void vx_model_get_options(const vx_model *model, vx_model_options *opt);
 vx_error vx_model_set_options(vx_model *model, const vx_model_options *opt);
 
+/* The KV cache in pages of 8-bit codes with one scale per page, layer and kv
+ * head (include/vxh.h, "paged KV cache in 8 bits"): type VXH_KVQ_INT8 or
+ * VXH_KVQ_E4M3 and page 32, 64 or 128 tokens, or type 0 for the cache that
+ * vx_model_options says (the default; page is ignored).  A change drops the
+ * cache (cache_len 0).  A quarter of the fp32 cache's bytes; every forward,
+ * verify and prompt path takes it.  head_dim 32, 64, 96 or 128; not with
+ * kv_half.  k_cache/v_cache then hold the device addresses of layer 0's codes;
+ * vx_model_read_kv returns the values they stand for.  A token's stored row
+ * depends on the rows that share its page so far (a later, larger one rounds
+ * it again), so a batch and its tokens one at a time agree to the rounding of
+ * 8 bits only.  The reference keeps fp32 (src/model.c:404-411). */
+vx_error vx_model_set_kv_pages(vx_model *model, int type, int page);
+
 /* Batched verify: runs tokens[0..n) at positions cache_len.. like n calls of
  * vx_model_forward with one token each, but in batches of up to 16 rows, and
  * writes every token's logits to logits_all[n][n_vocab]. */

@@ -401,7 +401,9 @@ def test_attention_scores_far_apart(P, rows, H, KV):
     pool, table, row0 = ragged(rng, [n], [rows], page)
     for kind in (Q.INT8, Q.E4M3):
         dc, oc = filled(P, kind, page, pool, KV, hd, rng)
-        for qs in (1e-30, 40.0, 3000.0):
+        # (at 1e9 a score's own fp32 rounding is past every other score: 64 bits
+        # say which token wins, and no tolerance but the largest value's bounds it)
+        for qs in (1e9, 1e25, 1e-30, 40.0, 3000.0):
             q = (rng.normal(0, 1, (rows, H * hd)) * qs).astype(np.float32)
             check_attend(P, dc, oc, q, row0, [n], table, H, 0)
         q[1] = 0

@@ -1,8 +1,11 @@
 """Paged 8-bit KV cache, without a GPU: the handle's layout, the refusals of
-every entry point (arguments are checked before anything is launched), and the
-numpy oracle's codes against their definition."""
+every entry point (arguments are checked before anything is launched), what a
+model on pages allocates and gives back, and the numpy oracle's codes against
+their definition."""
 import ctypes as C
+import glob
 import os
+import re
 import subprocess
 
 import numpy as np
@@ -126,3 +129,71 @@ def test_oracle_codes_are_the_nearest():
     assert Q.nearest(np.array([0.5, 1.5, 2.5, -0.5]), Q.INT8).tolist() == [0, 2, 2, -0.0]
     # e4m3 steps of 1/4 between 2 and 4: ties go to the even mantissa
     assert Q.nearest(np.array([2.125, 2.375, 2.0 ** -10, 3 * 2.0 ** -10]), Q.E4M3).tolist() == [2.0, 2.5, 0.0, 2.0 ** -8]
+
+
+# --------------------------------------------------------------------------
+# a model's memory: host/*.c over a stand-in device layer that counts
+# --------------------------------------------------------------------------
+@pytest.fixture(scope="module")
+def H(tmp_path_factory):
+    from test_prefill_buffers import BODIES, PRELUDE
+    d = tmp_path_factory.mktemp("host")
+    text = re.sub(r"/\*.*?\*/", "", open(os.path.join(N.REPO, "include", "vxh.h")).read(), flags=re.S)
+    bodies = dict(BODIES)
+    bodies["vxh_kvq_alloc"] = """memset(c, 0, sizeof *c);
+    if (vxh_malloc(&c->k, 1000)) return VXH_ERR_ALLOC;
+    if (vxh_malloc(&c->v, 1000)) { vxh_free(c->k); memset(c, 0, sizeof *c); return VXH_ERR_ALLOC; }
+    return 0;"""
+    bodies["vxh_kvq_free"] = "vxh_free(c->k); vxh_free(c->v); memset(c, 0, sizeof *c); return 0;"
+    src = PRELUDE
+    for ret, name, args in re.findall(r"^(int|size_t|void|const char \*) ?(vxh_\w+)\(([^;]*)\);", text, flags=re.M):
+        src += "%s %s(%s) { %s }\n" % (ret, name, args, bodies.pop(name, "" if ret == "void" else "return 0;"))
+    assert not bodies, sorted(bodies)
+    (d / "stub.c").write_text(src)
+    so = str(d / "host.so")
+    subprocess.run(["gcc", "-std=gnu11", "-O1", "-shared", "-fPIC", "-I", os.path.join(N.REPO, "include"), "-o", so,
+                    str(d / "stub.c")] + sorted(glob.glob(os.path.join(N.REPO, "veltrix-engine_amd", "host", "*.c"))) +
+                   ["-lm", "-Wl,-z,defs"], check=True)
+    L = C.CDLL(so)
+    L.vx_model_create_synthetic.argtypes = [C.POINTER(N.VxModelConfig), C.POINTER(N.VxSynthSpec),
+                                            C.POINTER(C.POINTER(N.VxModelDev))]
+    L.vx_model_set_kv_pages.argtypes = [C.POINTER(N.VxModelDev), C.c_int, C.c_int]
+    L.vx_model_forward.argtypes = [C.POINTER(N.VxModelDev), N.i32p, C.c_int, N.f32p]
+    L.vx_model_destroy.argtypes = [C.POINTER(N.VxModelDev)]
+    return L
+
+
+def test_a_paged_model_returns_its_memory(H):
+    budget, used = (C.c_size_t.in_dll(H, n) for n in ("st_budget", "st_used"))
+    cfg = N.VxModelConfig()
+    cfg.n_layers, cfg.n_heads, cfg.n_kv_heads, cfg.n_embd = 3, 2, 2, 128
+    cfg.n_ff, cfg.n_vocab, cfg.n_ctx = 256, 64, 1000
+    spec = N.VxSynthSpec(seed=1, std=0.02, matrix_type=2, embd_type=2, output_type=2)
+    lg = np.zeros(64, np.float32)
+
+    def walk():
+        """Every kind of cache in turn; the return codes of the forwards."""
+        m = C.POINTER(N.VxModelDev)()
+        rc = [H.vx_model_create_synthetic(C.byref(cfg), C.byref(spec), C.byref(m))]
+        if rc[0] == 0:
+            for kind, n in ((1, 5), (0, 60), (2, 70), (1, 1), (1, 60)):
+                assert H.vx_model_set_kv_pages(m, kind, 32) == 0
+                rc.append(H.vx_model_forward(m, np.zeros(n, np.int32), n, lg))
+            H.vx_model_destroy(m)
+        return rc
+
+    budget.value = 1 << 40
+    start = used.value
+    assert walk() == [0] * 6
+    assert used.value == start
+    # and when memory ends anywhere on the way
+    m = C.POINTER(N.VxModelDev)()
+    assert H.vx_model_create_synthetic(C.byref(cfg), C.byref(spec), C.byref(m)) == 0
+    model = used.value - start
+    H.vx_model_destroy(m)
+    failed = 0
+    for extra in range(0, 3_000_000, 1500):
+        budget.value = start + model + extra
+        failed += any(walk())
+        assert used.value == start, extra
+    assert failed > 100

@@ -140,6 +140,20 @@ __device__ __forceinline__ float vx_max8(const vx_f32x4 (&S)[2])
                  fmaxf(fmaxf(S[1][0], S[1][1]), fmaxf(S[1][2], S[1][3])));
 }
 
+// Scores S cs less their reference, each product rounded before the difference:
+// past VX_KVQ_FAR a fused one would leave the largest score above its own
+// rounded reference by more than a probability's range.
+#define VX_KVQ_FAR 0x1p20f
+__device__ __forceinline__ void vx_kvq_far(vx_f32x4 (&S)[2], float cs, float ref)
+{
+#pragma clang fp contract(off)
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const float p = S[e >> 2][e & 3] * cs;
+        S[e >> 2][e & 3] = p - ref;
+    }
+}
+
 __device__ __forceinline__ vx_f32x4 vx_mfma(vx_half8 a, vx_half8 b, vx_f32x4 c)
 {
     vx_f32x4 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);

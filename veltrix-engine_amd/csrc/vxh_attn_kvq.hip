@@ -364,7 +364,7 @@ __global__ __launch_bounds__(AK_THREADS, 3) void vx_attention_kvq_kernel(
             S[1] += L[1];
             const int t0 = 32 * g + 4 * g4;
             if (32 * g + 32 > lo || none) vx_kvq_mask(S, t0, none ? 0 : lim);
-            const float cs = fmaxf(qs * ksc, 1e-37f);         // -inf must not meet a zero
+            float cs = fmaxf(qs * ksc, 1e-37f);         // -inf must not meet a zero
             const float nm = fmaxf(m, vx_max_x32(vx_max_x16(vx_max8(S))) * cs), ref = nm == -INFINITY ? 0.0f : nm;
             if (__any(nm > m)) {
                 const float f = __builtin_amdgcn_exp2f(m - ref);
@@ -374,7 +374,12 @@ __global__ __launch_bounds__(AK_THREADS, 3) void vx_attention_kvq_kernel(
                 m = nm;
             }
             // probabilities times 2^14: their low parts stay normal numbers
-            const float sub = 14.0f - ref;
+            float sub = 14.0f - ref;
+            if (__any(fabsf(ref) > VX_KVQ_FAR)) {
+                vx_kvq_far(S, cs, ref);
+                cs = 1.0f;
+                sub = 14.0f;
+            }
             vx_half2 h[4], w[4];
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {

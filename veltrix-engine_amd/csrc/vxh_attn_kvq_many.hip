@@ -211,7 +211,7 @@ __global__ __launch_bounds__(256 * SK, 4) void vx_attention_kvq_many_kernel(vx_k
                 r = vsc * inv_U;
             }
             if (32 * g + 32 > lo || none) vx_kvq_mask(S, 32 * g + 4 * g4, none ? 0 : lim);
-            const float cs = fmaxf(qs * ksc, 1e-37f);  // -inf must not meet a zero
+            float cs = fmaxf(qs * ksc, 1e-37f);               // -inf must not meet a zero
             // the reference follows the maximum when that is 2^4 past it
             const float nm = vx_max_x32(vx_max_x16(vx_max8(S))) * cs;
             if (__any(nm > m + AM_SLACK) || fo != 1.0f) {
@@ -222,7 +222,13 @@ __global__ __launch_bounds__(256 * SK, 4) void vx_attention_kvq_many_kernel(vx_k
                 m = to;
             }
             // probabilities times 2^11: their low parts stay normal numbers
-            const float sub = 11.0f - (m == -INFINITY ? 0.0f : m);
+            const float ref = m == -INFINITY ? 0.0f : m;
+            float sub = 11.0f - ref;
+            if (__any(fabsf(ref) > VX_KVQ_FAR)) {
+                vx_kvq_far(S, cs, ref);
+                cs = 1.0f;
+                sub = 11.0f;
+            }
             vx_half2 h[4], w[4];
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {

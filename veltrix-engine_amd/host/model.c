@@ -162,11 +162,39 @@ static void pf_free(vx_dev *d)
 {
     vxh_free(d->pf_tok); vxh_free(d->pf_x); vxh_free(d->pf_qkv);
     vxh_free(d->pf_q); vxh_free(d->pf_att); vxh_free(d->pf_gu); vxh_free(d->pf_px);
+    vxh_free(d->pf_k); vxh_free(d->pf_v);
     d->pf_tok = NULL;
+    d->pf_k = d->pf_v = NULL;
     d->pf_x = d->pf_qkv = d->pf_q = d->pf_att = d->pf_gu = NULL;
     d->pf_px = NULL;
     vxh_workspace_free(&d->pf_ws);
     d->pf_rows = 0;
+}
+
+static void kvq_free(vx_dev *d)
+{
+    const int L = d->n_layers > 0 ? d->n_layers : 1;
+    for (int l = 0; d->kvq && l < L; l++) vxh_kvq_free(&d->kvq[l]);
+    free(d->kvq);
+    vxh_free(d->kvq_ids); vxh_free(d->kvq_table); vxh_free(d->kvq_step);
+    vxh_free(d->kvq_pos); vxh_free(d->kvq_slot); vxh_free(d->kvq_k); vxh_free(d->kvq_v);
+    d->kvq = NULL;
+    d->kvq_ids = d->kvq_table = d->kvq_step = d->kvq_pos = d->kvq_slot = NULL;
+    d->kvq_k = d->kvq_v = NULL;
+}
+
+/* Drops the KV cache, whichever kind it is; the next forward allocates one. */
+static void kv_drop(vx_model *m)
+{
+    vx_dev *d = vx_dev_of(m);
+    if (!d->kvq) {
+        vxh_free(m->k_cache);
+        vxh_free(m->v_cache);
+    }
+    kvq_free(d);
+    m->k_cache = m->v_cache = NULL;
+    m->cache_len = 0;
+    d->kv_gen++;
 }
 
 static void dev_free(vx_dev *d)
@@ -286,33 +314,21 @@ static vx_error dev_alloc_workspace(vx_dev *d, int n_ctx, int cap)
 {
     const int B = VX_MAX_BATCH;
     size_t an = vxh_attention_workspace_floats(B, n_ctx, cap, d->n_heads, d->n_kv, d->hd);
+    if (d->kvq_type) {
+        size_t qn = vxh_attention_kvq_workspace_floats(VX_PF_ROWS, 1, d->n_heads, d->n_kv, d->hd);
+        if (qn > an) an = qn;
+    }
     if (d->ws.part && d->ws.part_floats >= an) return VX_OK;
     vxh_workspace_free(&d->ws);
     TRY(vxh_workspace_alloc(&d->ws, 32, an));
     return VX_OK;
 }
 
-vx_error vx_dev_ensure_kv(vx_model *m)
+/* What a cache of n_ctx positions needs beside it: the RoPE tables and the
+ * attention's workspace. */
+static vx_error kv_tables(vx_model *m, int n_ctx)
 {
     vx_dev *d = vx_dev_of(m);
-    int n_ctx = m->config.n_ctx > 0 ? m->config.n_ctx : 4096;
-    if (m->k_cache && d->n_ctx_alloc == n_ctx) return VX_OK;
-    if (m->k_cache) {
-        /* n_ctx changed after the first forward: the reference keeps its
-         * first allocation; so does this engine */
-        return VX_OK;
-    }
-    size_t per = (size_t)(d->n_layers > 0 ? d->n_layers : 1) * n_ctx * d->kvd;
-    const size_t esz = d->opt.kv_half ? 2 : sizeof(float);   /* kvd is even: whole floats */
-    if ((size_t)n_ctx * d->kvd * esz > 0xFFFFFFFFull) {
-        /* the attention kernels address a layer's rows with 32-bit offsets */
-        vx_set_error("KV cache of %d positions x %d exceeds 4 GiB per layer", n_ctx, d->kvd);
-        return VX_ERR_UNSUPPORTED;
-    }
-    TRY(vxh_malloc((void **)&m->k_cache, per * esz));
-    TRY(vxh_malloc((void **)&m->v_cache, per * esz));
-    TRY(vxh_fill_f32(m->k_cache, 0.0f, per * esz / sizeof(float), d->stream));
-    TRY(vxh_fill_f32(m->v_cache, 0.0f, per * esz / sizeof(float), d->stream));
     d->n_ctx_alloc = n_ctx;
     d->kv_gen++;
     /* RoPE angle table for positions 0..n_ctx, computed like the reference
@@ -343,6 +359,70 @@ vx_error vx_dev_ensure_kv(vx_model *m)
     if (e != VX_OK) return e;
     TRY(vxh_stream_sync(d->stream));
     return VX_OK;
+}
+
+/* ints of a forward's step: len, add, len_out, row0[2], counts[4] */
+enum { KVQ_LEN = 0, KVQ_ADD = 1, KVQ_OUT = 2, KVQ_ROW0 = 3, KVQ_COUNTS = 5, KVQ_STEP_INTS = 9 };
+
+static vx_error kvq_alloc(vx_model *m, int n_ctx)
+{
+    vx_dev *d = vx_dev_of(m);
+    const int L = d->n_layers > 0 ? d->n_layers : 1, B = VX_MAX_BATCH;
+    d->kvq_pages = (n_ctx + d->kvq_page - 1) / d->kvq_page;
+    const size_t n_slots = (size_t)d->kvq_pages * d->kvq_page;
+    d->kvq = (vxh_kvq *)calloc((size_t)L, sizeof(vxh_kvq));
+    int *ids = (int *)malloc(sizeof(int) * n_slots);
+    if (!d->kvq || !ids) { free(ids); return VX_ERR_MEMORY; }
+    for (size_t i = 0; i < n_slots; i++) ids[i] = (int)i;
+    int rc = VXH_OK;
+    for (int l = 0; l < L && !rc; l++)
+        rc = vxh_kvq_alloc(&d->kvq[l], d->kvq_type, d->kvq_page, d->kvq_pages, d->n_kv, d->hd);
+    if (!rc) rc = vxh_malloc((void **)&d->kvq_ids, sizeof(int) * n_slots);
+    if (!rc) rc = vxh_upload(d->kvq_ids, ids, sizeof(int) * n_slots, d->stream);
+    if (!rc) rc = vxh_malloc((void **)&d->kvq_table, sizeof(int) * (size_t)d->kvq_pages);
+    if (!rc) rc = vxh_upload(d->kvq_table, ids, sizeof(int) * (size_t)d->kvq_pages, d->stream);
+    free(ids);
+    if (!rc) rc = vxh_malloc((void **)&d->kvq_step, sizeof(int) * KVQ_STEP_INTS);
+    if (!rc) rc = vxh_malloc((void **)&d->kvq_pos, sizeof(int) * VX_PF_ROWS);
+    if (!rc) rc = vxh_malloc((void **)&d->kvq_slot, sizeof(int) * VX_PF_ROWS);
+    if (!rc) rc = vxh_malloc((void **)&d->kvq_k, sizeof(float) * B * (size_t)d->kvd);
+    if (!rc) rc = vxh_malloc((void **)&d->kvq_v, sizeof(float) * B * (size_t)d->kvd);
+    m->k_cache = (float *)d->kvq[0].k;
+    m->v_cache = (float *)d->kvq[0].v;
+    return vx_from_vxh(rc);
+}
+
+static vx_error kv_alloc(vx_model *m, int n_ctx)
+{
+    vx_dev *d = vx_dev_of(m);
+    size_t per = (size_t)(d->n_layers > 0 ? d->n_layers : 1) * n_ctx * d->kvd;
+    const size_t esz = d->opt.kv_half ? 2 : sizeof(float);   /* kvd is even: whole floats */
+    if ((size_t)n_ctx * d->kvd * esz > 0xFFFFFFFFull) {
+        /* the attention kernels address a layer's rows with 32-bit offsets */
+        vx_set_error("KV cache of %d positions x %d exceeds 4 GiB per layer", n_ctx, d->kvd);
+        return VX_ERR_UNSUPPORTED;
+    }
+    TRY(vxh_malloc((void **)&m->k_cache, per * esz));
+    TRY(vxh_malloc((void **)&m->v_cache, per * esz));
+    TRY(vxh_fill_f32(m->k_cache, 0.0f, per * esz / sizeof(float), d->stream));
+    TRY(vxh_fill_f32(m->v_cache, 0.0f, per * esz / sizeof(float), d->stream));
+    return VX_OK;
+}
+
+vx_error vx_dev_ensure_kv(vx_model *m)
+{
+    vx_dev *d = vx_dev_of(m);
+    int n_ctx = m->config.n_ctx > 0 ? m->config.n_ctx : 4096;
+    if (m->k_cache && d->n_ctx_alloc == n_ctx) return VX_OK;
+    if (m->k_cache) {
+        /* n_ctx changed after the first forward: the reference keeps its
+         * first allocation; so does this engine */
+        return VX_OK;
+    }
+    vx_error e = d->kvq_type ? kvq_alloc(m, n_ctx) : kv_alloc(m, n_ctx);
+    if (e == VX_OK) e = kv_tables(m, n_ctx);
+    if (e != VX_OK) kv_drop(m);        /* nothing half made is left to a later forward */
+    return e;
 }
 
 /* --------------------------------------------------------------------------- */
@@ -646,8 +726,7 @@ void vx_model_destroy(vx_model *m)
     vx_dev *d = vx_dev_of(m);
     if (d) {
         vxh_stream_sync(d->stream);
-        vxh_free(m->k_cache);
-        vxh_free(m->v_cache);
+        kv_drop(m);
         dev_free(d);
     }
     free_host(m);
@@ -677,6 +756,10 @@ vx_error vx_model_set_options(vx_model *m, const vx_model_options *opt)
         return VX_ERR_PARAM;
     if (opt->kv_half != 0 && opt->kv_half != 1) return VX_ERR_PARAM;
     if (opt->prefill_min_rows < 0) return VX_ERR_PARAM;
+    if (opt->kv_half && d->kvq_type) {
+        vx_set_error("fp16 KV cache: the model's cache is paged (vx_model_set_kv_pages)");
+        return VX_ERR_UNSUPPORTED;
+    }
     if (opt->kv_half) {
         /* every forward must take the q|k|v attention kernel, the only one
          * with an fp16 cache */
@@ -694,14 +777,30 @@ vx_error vx_model_set_options(vx_model *m, const vx_model_options *opt)
     if (kv_changed && m->k_cache) {
         /* a cache of the other element type: dropped, allocated again by the next forward */
         TRY(vxh_stream_sync(d->stream));
-        vxh_free(m->k_cache);
-        vxh_free(m->v_cache);
-        m->k_cache = m->v_cache = NULL;
-        m->cache_len = 0;
-        d->kv_gen++;
+        kv_drop(m);
     }
     d->opt = *opt;   /* the prefill workspace follows the cap on its next use (pf_alloc) */
     if (cap_changed && m->k_cache) return dev_alloc_workspace(d, d->n_ctx_alloc, d->opt.attn_cap);
+    return VX_OK;
+}
+
+vx_error vx_model_set_kv_pages(vx_model *m, int type, int page)
+{
+    vx_dev *d = vx_dev_of(m);
+    if (!d) return VX_ERR_PARAM;
+    if (type == 0) page = 0;
+    else if ((type != VXH_KVQ_INT8 && type != VXH_KVQ_E4M3) || (page != 32 && page != 64 && page != 128))
+        return VX_ERR_PARAM;
+    if (type && (d->opt.kv_half || d->hd % 32 || d->hd > 128)) {
+        vx_set_error("paged KV cache: needs head_dim 32, 64, 96 or 128 (%d) and kv_half 0", d->hd);
+        return VX_ERR_UNSUPPORTED;
+    }
+    if (type == d->kvq_type && page == d->kvq_page) return VX_OK;
+    TRY(vxh_stream_sync(d->stream));
+    if (m->k_cache) kv_drop(m);
+    pf_free(d);                        /* a prompt chunk's buffers follow the kind of cache */
+    d->kvq_type = type;
+    d->kvq_page = page;
     return VX_OK;
 }
 
@@ -867,6 +966,52 @@ static vx_error pgemm(vx_dev *d, const vxh_qmat *W, const vxh_pro *p, int M, dou
     return VX_OK;
 }
 
+/* ---- the paged 8-bit cache ----------------------------------------------------- */
+static int fill_int(int *dst, int value, vxh_stream s)
+{
+    float f;                           /* the same 32 bits */
+    memcpy(&f, &value, sizeof f);
+    return vxh_fill_f32((float *)dst, f, 1, s);
+}
+
+/* The pages, slots and lengths of a forward of M rows at n_past.., for all of
+ * its layers.  One row may stand past the context: it takes the last position,
+ * as the reference's clamp does (src/model.c:279-286). */
+static vx_error kvq_begin(vx_dev *d, int M, int n_past)
+{
+    const int n_ctx = d->n_ctx_alloc;
+    if (n_past + M > n_ctx) {
+        if (M > 1) {
+            vx_set_error("paged KV cache: %d rows at %d pass the context of %d", M, n_past, n_ctx);
+            return VX_ERR_PARAM;
+        }
+        n_past = n_ctx - 1;
+    }
+    const int have = (n_past + d->kvq_page - 1) / d->kvq_page;
+    int *st = d->kvq_step;
+    TRY(fill_int(st + KVQ_LEN, n_past, d->stream));
+    TRY(fill_int(st + KVQ_ADD, M, d->stream));
+    TRY(vxh_page_tables(st + KVQ_LEN, st + KVQ_ADD, 1, d->kvq_page, d->kvq_ids + have, d->kvq_pages - have,
+                        d->kvq_table, d->kvq_pages, st + KVQ_OUT, st + KVQ_ROW0, d->kvq_pos, d->kvq_slot, M,
+                        st + KVQ_COUNTS, d->stream));
+    return VX_OK;
+}
+
+/* Layer l's rotated k and v rows into its pages, then its attention. */
+static vx_error kvq_attend(vx_dev *d, int l, int M, const float *k, const float *v, const float *q, float *out)
+{
+    const int *st = d->kvq_step;
+    TRY(vxh_kvq_write(&d->kvq[l], k, d->kvd, v, d->kvd, d->kvq_slot, M, d->stream));
+    TRY(vxh_attention_kvq(q, d->d, st + KVQ_ROW0, st + KVQ_OUT, 1, M, M, d->kvq_table, d->kvq_pages, d->n_heads,
+                          &d->kvq[l], d->opt.attn_cap, out, d->d, &d->ws, d->stream));
+    return VX_OK;
+}
+
+/* The RoPE tables from position n_past on: a rotation that writes its rows to
+ * a forward's own buffers counts them from zero. */
+#define ROPE_FROM(d, n_past) \
+    (d)->rope_cos + (size_t)(n_past) * ((d)->hd / 2), (d)->rope_sin + (size_t)(n_past) * ((d)->hd / 2), (d)->n_pos - (n_past)
+
 /* Prologue forward: each GEMM builds its own input panel slice.
  *   QKV     t = x + acc_x (previous down projection) -> x2, panel attn_norm .* t
  *   RoPE    q|k|v = RoPE(acc_qkv / rms(t)), new k/v rows into the cache
@@ -894,8 +1039,10 @@ static vx_error forward_pro(vx_model *m, int M, int n_past, int logits_mode)
      * that take the q|k|v attention give every layer its own accumulators
      * (acc_dec), cleared here with the rest, so no launch of the forward
      * clears one */
-    const int attn_in_o = M <= VXH_PRO_ATTN_MAX_ROWS && d->hd % 4 == 0;
-    const int qkv_fast = M <= VXH_ATTN_QKV_FAST_ROWS && (d->hd == 64 || d->hd == 128);
+    const int paged = d->kvq_type != 0;
+    const int attn_in_o = !paged && M <= VXH_PRO_ATTN_MAX_ROWS && d->hd % 4 == 0;
+    const int qkv_fast = !paged && M <= VXH_ATTN_QKV_FAST_ROWS && (d->hd == 64 || d->hd == 128);
+    if (paged && (e = kvq_begin(d, M, n_past)) != VX_OK) return e;
     const int dec = attn_in_o || (qkv_fast && !d->opt.kv_half);
     /* the sums of squares and acc_x's rows (the previous prologue forward's
      * output GEMM may have left its last down projection in acc_x_rows of
@@ -925,7 +1072,7 @@ static vx_error forward_pro(vx_model *m, int M, int n_past, int logits_mode)
         vx_dev_layer *Ld = &d->layers[l];
         const int kvh = d->opt.kv_half;
         const size_t kv_off = (size_t)l * n_ctx * kvd;
-        float *kc = m->k_cache + kv_off, *vc = m->v_cache + kv_off;
+        float *kc = paged ? d->kvq_k : m->k_cache + kv_off, *vc = paged ? d->kvq_v : m->v_cache + kv_off;
         uint16_t *kh = (uint16_t *)m->k_cache + kv_off, *vh = (uint16_t *)m->v_cache + kv_off;
         memset(&p, 0, sizeof(p));
         p.kind = VXH_PRO_RESID;
@@ -968,6 +1115,12 @@ static vx_error forward_pro(vx_model *m, int M, int n_past, int logits_mode)
                 TRY(vxh_attention_qkv(d->acc_qkv, d->ld_qkv, SS(l, 0), dd, Ld->bq, Ld->bk, Ld->bv,
                                       d->rope_cos, d->rope_sin, d->n_pos, M, n_past, n_ctx, d->n_heads,
                                       d->n_kv, d->hd, d->opt.attn_cap, kc, vc, d->att, dd, &d->ws, s));
+            p.kind = VXH_PRO_ROWS;
+            p.x = d->att; p.ldx = dd;
+        } else if (paged) {
+            TRY(vxh_rope_kv_norm(d->acc_qkv, d->ld_qkv, M, 0, M, d->n_heads, d->n_kv, d->hd, Ld->bq, Ld->bk, Ld->bv,
+                                 ROPE_FROM(d, n_past), SS(l, 0), dd, d->q, kc, vc, s));
+            if ((e = kvq_attend(d, l, M, kc, vc, d->q, d->att)) != VX_OK) return e;
             p.kind = VXH_PRO_ROWS;
             p.x = d->att; p.ldx = dd;
         } else {
@@ -1090,6 +1243,8 @@ vx_error vx_dev_forward(vx_model *m, int M, int n_past, int logits_mode)
     vxh_stream s = d->stream;
     vx_error e;
 
+    const int paged = d->kvq_type != 0;
+    if (paged && (e = kvq_begin(d, M, n_past)) != VX_OK) return e;
     if ((d->acc_dirty || d->acc_x_rows) && (e = zero_acc(d)) != VX_OK) return e;
     d->acc_dirty = 1;
     if (d->has_embd) TRY(vxh_qmat_gather_rows(&d->embd, d->tok, M, vx_get_synthetic_weight_scale(), d->x, dd, s));
@@ -1097,18 +1252,24 @@ vx_error vx_dev_forward(vx_model *m, int M, int n_past, int logits_mode)
 
     for (int l = 0; l < d->n_layers; l++) {
         vx_dev_layer *Ld = &d->layers[l];
-        float *kc = m->k_cache + (size_t)l * n_ctx * kvd;
-        float *vc = m->v_cache + (size_t)l * n_ctx * kvd;
+        float *kc = paged ? d->kvq_k : m->k_cache + (size_t)l * n_ctx * kvd;
+        float *vc = paged ? d->kvq_v : m->v_cache + (size_t)l * n_ctx * kvd;
         /* x += previous down projection; attention RMSNorm; QKV tail = x[0..3] */
         TRY(vxh_resid_rmsnorm_panel(d->x, dd, d->acc_x, dd, M, dd, Ld->attn_norm, avx2, 1, &d->pan_d,
                                     (avx2 && Ld->has_o) ? d->xn : NULL, dd, s));
         if ((e = gemm(d, &Ld->wqkv, &d->pan_d, M, d->acc_qkv, d->ld_qkv, dd + 2 * kvd, VX_PROF_QKV,
                       dd + 2 * kvd)))
             return e;
-        TRY(vxh_rope_kv(d->acc_qkv, d->ld_qkv, M, n_past, n_ctx, d->n_heads, d->n_kv, d->hd, Ld->bq,
-                        Ld->bk, Ld->bv, d->rope_cos, d->rope_sin, d->n_pos, d->q, kc, vc, s));
-        TRY(vxh_attention(d->q, M, n_past, n_ctx, d->n_heads, d->n_kv, d->hd, d->opt.attn_cap, kc, vc,
-                          d->att, dd, &d->ws, s));
+        if (paged) {
+            TRY(vxh_rope_kv(d->acc_qkv, d->ld_qkv, M, 0, M, d->n_heads, d->n_kv, d->hd, Ld->bq, Ld->bk, Ld->bv,
+                            ROPE_FROM(d, n_past), d->q, kc, vc, s));
+            if ((e = kvq_attend(d, l, M, kc, vc, d->q, d->att)) != VX_OK) return e;
+        } else {
+            TRY(vxh_rope_kv(d->acc_qkv, d->ld_qkv, M, n_past, n_ctx, d->n_heads, d->n_kv, d->hd, Ld->bq,
+                            Ld->bk, Ld->bv, d->rope_cos, d->rope_sin, d->n_pos, d->q, kc, vc, s));
+            TRY(vxh_attention(d->q, M, n_past, n_ctx, d->n_heads, d->n_kv, d->hd, d->opt.attn_cap, kc, vc,
+                              d->att, dd, &d->ws, s));
+        }
         if (Ld->has_o) {
             /* attn_o's x86-build tail is the normed x (src/model.c:426, :544) */
             TRY(vxh_prep_panel(&d->pan_d, d->att, dd, M, dd, avx2, d->xn, dd, s));
@@ -1182,6 +1343,10 @@ static vx_error pf_alloc_rows(vx_dev *d, int rows)
     TRY(vxh_malloc((void **)&d->pf_att, sizeof(float) * R * d->d));
     TRY(vxh_malloc((void **)&d->pf_gu, sizeof(float) * R * d->ld_gu));
     TRY(vxh_malloc(&d->pf_px, vxh_rows_panel_bytes(rows, d->F > d->d ? d->F : d->d)));
+    if (d->kvq_type) {
+        TRY(vxh_malloc((void **)&d->pf_k, sizeof(float) * R * d->kvd));
+        TRY(vxh_malloc((void **)&d->pf_v, sizeof(float) * R * d->kvd));
+    }
     vx_error e = pf_ws_alloc(d, rows);
     if (e == VX_OK) d->pf_rows = rows;
     return e;
@@ -1243,19 +1408,28 @@ static vx_error forward_prefill(vx_model *m, const int *tokens, int M, int n_pas
     const int dd = d->d, kvd = d->kvd, n_ctx = d->n_ctx_alloc;
     vxh_stream s = d->stream;
     vx_error e;
+    const int paged = d->kvq_type != 0;
+    if (paged && (e = kvq_begin(d, M, n_past)) != VX_OK) return e;
     TRY(vxh_upload(d->pf_tok, tokens, sizeof(int) * (size_t)M, s));
     if (d->has_embd) TRY(vxh_qmat_gather_rows(&d->embd, d->pf_tok, M, vx_get_synthetic_weight_scale(), d->pf_x, dd, s));
     else TRY(vxh_fill_f32(d->pf_x, 0.0f, (size_t)M * dd, s));
     for (int l = 0; l < d->n_layers; l++) {
         vx_dev_layer *Ld = &d->layers[l];
-        float *kc = m->k_cache + (size_t)l * n_ctx * kvd, *vc = m->v_cache + (size_t)l * n_ctx * kvd;
+        const size_t kv_off = (size_t)l * n_ctx * kvd;
+        float *kc = paged ? d->pf_k : m->k_cache + kv_off, *vc = paged ? d->pf_v : m->v_cache + kv_off;
         TRY(vxh_rmsnorm_rows_panel(d->pf_x, dd, M, dd, Ld->attn_norm, d->pf_px, s));
         TRY(vxh_gemm_rows(&Ld->wqkv, d->pf_px, M, d->pf_qkv, d->ld_qkv, dd + 2 * kvd, NULL, 0,
                           scale_for(d, Ld->wqkv.type), s));
-        TRY(vxh_rope_kv_rows(d->pf_qkv, d->ld_qkv, M, n_past, n_ctx, d->n_heads, d->n_kv, d->hd, Ld->bq, Ld->bk,
-                             Ld->bv, d->rope_cos, d->rope_sin, d->n_pos, d->pf_q, dd, kc, vc, s));
-        TRY(vxh_attention_rows(d->pf_q, M, n_past, n_ctx, d->n_heads, d->n_kv, d->hd, d->opt.attn_cap, kc, vc,
-                               d->pf_att, dd, &d->pf_ws, s));
+        if (paged) {
+            TRY(vxh_rope_kv_rows(d->pf_qkv, d->ld_qkv, M, 0, M, d->n_heads, d->n_kv, d->hd, Ld->bq, Ld->bk, Ld->bv,
+                                 ROPE_FROM(d, n_past), d->pf_q, dd, kc, vc, s));
+            if ((e = kvq_attend(d, l, M, kc, vc, d->pf_q, d->pf_att)) != VX_OK) return e;
+        } else {
+            TRY(vxh_rope_kv_rows(d->pf_qkv, d->ld_qkv, M, n_past, n_ctx, d->n_heads, d->n_kv, d->hd, Ld->bq, Ld->bk,
+                                 Ld->bv, d->rope_cos, d->rope_sin, d->n_pos, d->pf_q, dd, kc, vc, s));
+            TRY(vxh_attention_rows(d->pf_q, M, n_past, n_ctx, d->n_heads, d->n_kv, d->hd, d->opt.attn_cap, kc, vc,
+                                   d->pf_att, dd, &d->pf_ws, s));
+        }
         if (Ld->has_o) {
             TRY(vxh_rows_panel(d->pf_att, dd, M, dd, d->pf_px, s));
             TRY(vxh_gemm_rows(&Ld->wo, d->pf_px, M, d->pf_x, dd, dd, d->pf_x, dd, scale_for(d, Ld->wo.type), s));
@@ -1410,11 +1584,30 @@ vx_error vx_model_read_tensor(const vx_model *m, const char *name, void *dst, si
     return VX_OK;
 }
 
+static vx_error kvq_read_rows(vx_dev *d, int layer, int n, float *k, float *v)
+{
+    enum { ROWS = 512 };
+    float *dk = NULL, *dv = NULL;
+    const size_t row = sizeof(float) * (size_t)d->kvd;
+    int rc = vxh_malloc((void **)&dk, ROWS * row);
+    if (!rc) rc = vxh_malloc((void **)&dv, ROWS * row);
+    for (int r = 0; r < n && !rc; r += ROWS) {
+        const int c = n - r < ROWS ? n - r : ROWS;
+        rc = vxh_kvq_read(&d->kvq[layer], d->kvq_ids + r, c, dk, d->kvd, dv, d->kvd, d->stream);
+        if (!rc && k) rc = vxh_download(k + (size_t)r * d->kvd, dk, c * row, d->stream);
+        if (!rc && v) rc = vxh_download(v + (size_t)r * d->kvd, dv, c * row, d->stream);
+    }
+    vxh_free(dk);
+    vxh_free(dv);
+    return vx_from_vxh(rc);
+}
+
 vx_error vx_model_read_kv(const vx_model *m, int layer, int n, float *k, float *v)
 {
     vx_dev *d = vx_dev_of(m);
     if (!d || !m->k_cache || layer < 0 || layer >= d->n_layers || n < 0 || n > d->n_ctx_alloc)
         return VX_ERR_PARAM;
+    if (d->kvq) return kvq_read_rows(d, layer, n, k, v);
     size_t off = (size_t)layer * d->n_ctx_alloc * d->kvd;
     size_t cnt = (size_t)n * d->kvd;
     if (d->opt.kv_half) {

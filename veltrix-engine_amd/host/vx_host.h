@@ -122,6 +122,17 @@ typedef struct vx_dev {
     float *pf_x, *pf_qkv, *pf_q, *pf_att, *pf_gu;
     void *pf_px;                       /* rows panel of the GEMM input (vxh_rows_panel) */
     vxh_workspace pf_ws;
+    /* paged 8-bit KV cache (vx_model_set_kv_pages): a pool per layer, one page
+     * table for all of them (page i of a layer holds tokens i * kvq_page ..) */
+    int kvq_type, kvq_page;            /* 0: the cache of opt                     */
+    vxh_kvq *kvq;                      /* [n_layers], allocated with the cache    */
+    int kvq_pages;
+    int *kvq_ids;                      /* 0, 1, ..: the pages in order, and every slot */
+    int *kvq_table;                    /* [kvq_pages]                             */
+    int *kvq_step;                     /* KVQ_STEP_INTS: a forward's lengths      */
+    int *kvq_pos, *kvq_slot;           /* [VX_PF_ROWS]                            */
+    float *kvq_k, *kvq_v;              /* a forward's rotated rows, [VX_MAX_BATCH][kvd] */
+    float *pf_k, *pf_v;                /* the same for a prompt chunk             */
     /* GEMM profiling (vx_model_set_profiling) */
     int prof_on;                       /* 0: off; n: every n-th launch per class   */
     int prof_tick[VX_PROF_N];
