@@ -557,6 +557,9 @@ int vxh_kvq_read(const vxh_kvq *c, const int *slot, int R, float *k, int ldk, fl
  * last request stay as they were.  What the cache holds past the positions a
  * request's rows read may be anything; a table entry that is no page counts as
  * positions nobody reads, and lengths past ld_table pages end there.
+ * Scores, sums and results are held in fp32, queries and probabilities as two
+ * fp16 parts of 22 bits; values whose scale is 2^60 below the largest that
+ * their row reads may count as zeros.
  * max_seq_rows is the largest number of rows a request is expected to have;
  * only speed depends on it.  q and out 16-byte aligned, ldq and ld_out
  * multiples of 4.  The partial results of requests cut into segments live in

@@ -118,6 +118,27 @@ def test_attention_refuses(P, over):
     assert b"attention_kvq" in P.vxh_last_error()
 
 
+@pytest.mark.parametrize("over", [dict(k=(1 << 20) + 4), dict(v=(1 << 20) + 8), dict(ks=(1 << 20) + 2),
+                                  dict(vs=(1 << 20) + 1), dict(n_kv_heads=1 << 26)])
+def test_handles_of_arrays_that_cannot_be_loaded(P, over):
+    """Arrays off their alignment, and heads whose row passes 32 bits."""
+    c = C.byref(handle(**over))
+    ws = Q.Workspace(acc=1 << 20, part=1 << 20, part_floats=1 << 40)
+    big = 0x7FFFFFFC
+    assert P.vxh_kvq_write(c, PTR, big, PTR, big, PTR, 4, None) == -3
+    assert P.vxh_kvq_read(c, PTR, 4, PTR, big, PTR, big, None) == -3
+    assert P.vxh_attention_kvq(PTR, big, PTR, PTR, 1, 1, 1, PTR, 4, 1 << 26, c, 0, PTR, big, C.byref(ws), None) == -3
+
+
+def test_counts_that_pass_32_bits_are_refused(P):
+    ws = C.byref(Q.Workspace(acc=1 << 20, part=1 << 20, part_floats=1 << 40))
+    big = 0x7FFFFFFC
+    for heads, rows in ((1 << 26, 1), (1 << 25, 1), (1 << 24, 128), (8192, 1 << 18)):
+        assert P.vxh_attention_kvq(*attend_args(heads=heads, rows=rows, ldq=big, ld_out=big, ws=ws)) == -3
+    assert P.vxh_page_tables(*tables_args(page=128, ld=1 << 24)) == -3
+    assert P.vxh_page_tables(*tables_args(page=32, ld=1 << 26)) == -3
+
+
 def test_oracle_codes_are_the_nearest():
     """nearest() against a search over every code."""
     rng = np.random.default_rng(5)

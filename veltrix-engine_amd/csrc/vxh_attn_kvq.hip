@@ -18,6 +18,7 @@
 #define AK_SMALL 8               // tiles of up to this many groups take a wavefront each
 #define AK_SNAP 12               // most groups a piece's end moves to a tile's
 #define AK_FEW 64                // queries per kv head up to which a request is this kernel's
+#define AK_P 16384.0f            // what a probability is times in the matrix products
 #define AK_JOIN 8                // parts whose loads are in flight together
 #define AK_BLOCK 16              // parts one workgroup joins
 
@@ -346,7 +347,7 @@ __global__ __launch_bounds__(AK_THREADS, 3) void vx_attention_kvq_kernel(
             const uint8_t *kn = kc + base + lane * 16, *vn = vc + base + lane * 16;
             const size_t hp = (size_t)max(page, 0) * a.n_kv + kvh;
             const bool none = page < 0;
-            const float ksc = none ? 0.0f : ks[hp], vsc = none ? 0.0f : vs[hp];
+            const float ksc = none ? 0.0f : ks[hp], vsc = none ? 0.0f : vs[hp] * (1.0f / AK_P);
             page = next;
             vx_f32x4 S[2], L[2];                              // of the high and of the low parts
 #pragma unroll
@@ -373,7 +374,7 @@ __global__ __launch_bounds__(AK_THREADS, 3) void vx_attention_kvq_kernel(
                 for (int d = 0; d < ND; d++) O[d] *= f;
                 m = nm;
             }
-            // probabilities times 2^14: their low parts stay normal numbers
+            // probabilities times 2^14 (AK_P): their low parts stay normal numbers
             float sub = 14.0f - ref;
             if (__any(fabsf(ref) > VX_KVQ_FAR)) {
                 vx_kvq_far(S, cs, ref);
@@ -409,7 +410,7 @@ __global__ __launch_bounds__(AK_THREADS, 3) void vx_attention_kvq_kernel(
         }
 
         auto finish = [&](int qi, int d, vx_f32x4 o, float sum) {
-            const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+            const float inv = sum != 0.0f ? AK_P / sum : 0.0f;
             *(vx_f32x4 *)(out + (size_t)(s.row + qi / a.G) * c.ld_out + (size_t)(kvh * a.G + qi % a.G) * HD + d) = o * inv;
         };
         l = vx_sum_x32(vx_sum_x16(l));
@@ -514,10 +515,11 @@ extern "C" int vxh_attention_kvq(const float *q, int ldq, const int *row0, const
                                  int cap, float *out, int ld_out, vxh_workspace *ws, vxh_stream s)
 {
     if (const char *bad = vx_kvq_bad(c)) return vxh_fail(VXH_ERR_PARAM, "attention_kvq: %s", bad);
-    const int w = n_heads * c->head_dim;
+    // (no row count times head count passes 32 bits in the kernels)
+    const int64_t w = (int64_t)n_heads * c->head_dim;
     if (!q || !row0 || !len || !table || !out || !ws || !ws->acc || !ws->part || n_seqs < 1 || n_seqs > VXH_PAGE_MAX_SEQS ||
         max_rows < 1 || max_rows > VXH_PAGE_MAX_ROWS || max_seq_rows < 1 || ld_table < 1 || cap < 0 || n_heads < 1 ||
-        n_heads % c->n_kv_heads || ldq < w || ldq % 4 || ld_out < w || ld_out % 4 || ((uintptr_t)q & 15) ||
+        (int64_t)max_rows * n_heads > 0x7FFFFFFF || n_heads % c->n_kv_heads || ldq < w || ldq % 4 || ld_out < w || ld_out % 4 || ((uintptr_t)q & 15) ||
         ((uintptr_t)out & 15) ||
         ws->part_floats < vxh_attention_kvq_workspace_floats(max_rows, n_seqs, n_heads, c->n_kv_heads, c->head_dim))
         return vxh_fail(VXH_ERR_PARAM, "attention_kvq: %d requests, %d rows, %d/%d heads of %d (ld %d, %d)", n_seqs,

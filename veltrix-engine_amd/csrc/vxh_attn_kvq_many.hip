@@ -9,8 +9,8 @@
 // of the largest one met (U), so that P V sums up inside the MFMAs.
 #include "vxh_attn_kvq.h"
 
-
 #define AM_QT 64                 // queries of a tile
+#define AM_P 2048.0f             // what a probability is times in the matrix products
 #define AM_SLACK 4.0f            // powers of two a score may pass the reference by
 
 struct vx_kvq_unit {
@@ -221,7 +221,7 @@ __global__ __launch_bounds__(256 * SK, 4) void vx_attention_kvq_many_kernel(vx_k
                 for (int d = 0; d < ND; d++) O[d] *= f * fo;
                 m = to;
             }
-            // probabilities times 2^11: their low parts stay normal numbers
+            // probabilities times 2^11 (AM_P): their low parts stay normal numbers
             const float ref = m == -INFINITY ? 0.0f : m;
             float sub = 11.0f - ref;
             if (__any(fabsf(ref) > VX_KVQ_FAR)) {
@@ -255,7 +255,7 @@ __global__ __launch_bounds__(256 * SK, 4) void vx_attention_kvq_many_kernel(vx_k
     }
     l = vx_sum_x32(vx_sum_x16(l));
 #pragma unroll
-    for (int d = 0; d < ND; d++) O[d] *= U;
+    for (int d = 0; d < ND; d++) O[d] *= U * (1.0f / AM_P);
     if (strm > 0) {
         float *so = sh.o[strm - 1][16 * wave + n];
 #pragma unroll
@@ -283,7 +283,7 @@ __global__ __launch_bounds__(256 * SK, 4) void vx_attention_kvq_many_kernel(vx_k
         for (int d = 0; d < ND; d++) O[d] += *(const vx_f32x4 *)(so + 16 * d + 4 * g4) * f;
     }
     if (!ok) return;
-    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    const float inv = l != 0.0f ? AM_P / l : 0.0f;
     float *o = c.out + row * c.ld_out + col + 4 * g4;
 #pragma unroll
     for (int d = 0; d < ND; d++) *(vx_f32x4 *)(o + 16 * d) = O[d] * inv;

@@ -10,7 +10,11 @@ const char *vx_kvq_bad(const vxh_kvq *c)
     if (c->type != VXH_KVQ_INT8 && c->type != VXH_KVQ_E4M3) return "type";
     if (c->page != 32 && c->page != 64 && c->page != 128) return "page size";
     if (c->head_dim % 32 || c->head_dim < 32 || c->head_dim > 128) return "head_dim";
-    if (c->n_pages < 1 || c->n_kv_heads < 1 || (int64_t)c->n_pages * c->page > 0x7FFFFFFF) return "size";
+    if (c->n_pages < 1 || c->n_kv_heads < 1 || (int64_t)c->n_pages * c->page > 0x7FFFFFFF ||
+        (int64_t)c->n_kv_heads * c->head_dim > 0x3FFFFFFF)
+        return "size";
+    if (((uintptr_t)c->k & 15) || ((uintptr_t)c->v & 15) || ((uintptr_t)c->ks & 3) || ((uintptr_t)c->vs & 3))
+        return "alignment";
     return nullptr;
 }
 
@@ -18,7 +22,8 @@ extern "C" int vxh_kvq_alloc(vxh_kvq *c, int type, int page, int n_pages, int n_
 {
     if (!c) return vxh_fail(VXH_ERR_PARAM, "kvq_alloc: no handle");
     memset(c, 0, sizeof(*c));
-    vxh_kvq t = {type, page, n_pages, n_kv_heads, head_dim, c, c, (float *)c, (float *)c};
+    float *const some = (float *)16;                     // the arrays come once the rest is known to be good
+    vxh_kvq t = {type, page, n_pages, n_kv_heads, head_dim, some, some, some, some};
     if (const char *bad = vx_kvq_bad(&t))
         return vxh_fail(VXH_ERR_PARAM, "kvq_alloc: %s (type %d, %d pages of %d, %d heads of %d)", bad, type, n_pages,
                         page, n_kv_heads, head_dim);
@@ -143,7 +148,7 @@ __global__ __launch_bounds__(PT_THREADS) void vx_page_tables_kernel(
     };
     for (int i = first; ok && i < f_all; i += step) {
         const int b = find(s_new, i);
-        const int have = (max(len[b], 0) + mask) >> shift;
+        const int have = (int)(((int64_t)max(len[b], 0) + mask) >> shift);
         table[(size_t)b * ld_table + have + i - s_new[b]] = free_pages[i];
     }
     for (int r = first; r < max_rows; r += step) {
@@ -173,7 +178,7 @@ extern "C" int vxh_page_tables(const int *len, const int *add, int n_seqs, int p
     if (!len || !add || !table || !len_out || !row0 || !row_pos || !slot || !counts || (n_free > 0 && !free_pages))
         return vxh_fail(VXH_ERR_PARAM, "page_tables: missing array");
     if (n_seqs < 1 || n_seqs > VXH_PAGE_MAX_SEQS || (page != 32 && page != 64 && page != 128) || n_free < 0 ||
-        ld_table < 1 || max_rows < 1 || max_rows > VXH_PAGE_MAX_ROWS)
+        ld_table < 1 || (int64_t)ld_table * page > 0x7FFFFFFF || max_rows < 1 || max_rows > VXH_PAGE_MAX_ROWS)
         return vxh_fail(VXH_ERR_PARAM, "page_tables: %d requests, pages of %d, %d free, %d columns, %d rows", n_seqs,
                         page, n_free, ld_table, max_rows);
     const size_t nb = (size_t)n_seqs * sizeof(int);
