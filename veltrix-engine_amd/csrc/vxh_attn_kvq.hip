@@ -238,7 +238,7 @@ __device__ __forceinline__ void vx_kvq_join(const float *part, Slot slot, int i0
 // every fourth group and join in LDS; short tiles take a wavefront each.
 // ---------------------------------------------------------------------------
 template <int TYPE, int HD>
-__global__ __launch_bounds__(AK_THREADS, 3) void vx_attention_kvq_kernel(
+__global__ __launch_bounds__(AK_THREADS, 2) void vx_attention_kvq_kernel(
     vx_kvq_call c, const float *__restrict__ q, const int *__restrict__ table, const uint8_t *__restrict__ kc,
     const uint8_t *__restrict__ vc, const float *__restrict__ ks, const float *__restrict__ vs, float *__restrict__ out,
     float *__restrict__ part, unsigned *__restrict__ counter)
