@@ -202,8 +202,12 @@ extern "C" int vxh_page_tables(const int *len, const int *add, int n_seqs, int p
 // as whole 16-byte lanes, blended with the page's other tokens.
 // ---------------------------------------------------------------------------
 #define KW_THREADS 256
-#define KW_PIECES 256            // of the rows
+#define KW_PIECES 128            // of the rows
 #define KW_WG 2048               // workgroups; heads past that in turn
+
+// x is taken as new here: what follows from it is worked out again, not kept in
+// registers (16 items' conditions, for every part) from before the loop.
+#define KW_HERE(x) asm("" : "+v"(x))
 
 // Bytes of a word whose bits 0..3 are set in nib.
 __device__ __forceinline__ uint32_t vx_spread(uint32_t nib) { return (((nib & 15u) * 0x00204081u) & 0x01010101u) * 0xFFu; }
@@ -225,10 +229,21 @@ __global__ __launch_bounds__(KW_THREADS) void vx_kvq_write_kernel(vxh_kvq c, con
     auto token = [&](int it) { return (int)(((float)it + 0.5f) * per4); };
     auto page_of = [&](int sl) { return sl < 0 || (unsigned)(sl >> SHIFT) >= n_pages ? -1 : sl >> SHIFT; };
     const int r1 = min((int)(blockIdx.y + 1) * chunk, R);
-    for (int lead = blockIdx.y * chunk; lead < r1; lead++) {
-        // rows behind another of their page are that one's
-        const int page = page_of(slot[lead]);
-        if (page < 0 || (lead > 0 && page_of(slot[lead - 1]) == page)) continue;
+    uint64_t leads = 0;                                  // of 64 rows from base: those that may lead a page
+    int here = -1;                                       // the lane's row's page
+    for (int base = blockIdx.y * chunk - 64;;) {
+        if (!leads) {
+            // (a row behind another of its page is that one's)
+            base += 64;
+            if (base >= r1) break;
+            const int r = base + lane;
+            here = r < r1 ? page_of(slot[r]) : -1;
+            const int before = r < r1 && r > 0 ? page_of(slot[r - 1]) : -1;
+            leads = __ballot(here >= 0 && here != before);
+            continue;
+        }
+        const int at = __ffsll((unsigned long long)leads) - 1, lead = base + at, page = __builtin_amdgcn_readlane(here, at);
+        leads &= leads - 1;
         __syncthreads();
         if (tid == 0) s_first = R;
         for (int i = tid; i < P; i += KW_THREADS) s_src[i] = -1;
@@ -253,16 +268,22 @@ __global__ __launch_bounds__(KW_THREADS) void vx_kvq_write_kernel(vxh_kvq c, con
         // a part's rows, this thread's items of 4 dims; the next part's are on
         // their way while one is worked on
         float4 val[NI];
+        unsigned live = 0;                               // items whose token comes, a bit each
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            const int t = token(tid + i * KW_THREADS);
+            if (t < P && s_src[t] >= 0) live |= 1u << i;
+        }
         auto fetch = [&](int part) {
             const bool is_v = part >= c.n_kv_heads;
             const int ldx = is_v ? ldv : ldk;
             const float *x = is_v ? v + (part - c.n_kv_heads) * hd : k + part * hd;
+            KW_HERE(live);
 #pragma unroll
             for (int i = 0; i < NI; i++) {
                 const int it = tid + i * KW_THREADS, t = token(it);
-                const int src = t < P ? s_src[t] : -1;
                 val[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (src >= 0) val[i] = *(const float4 *)(x + (size_t)src * ldx + 4 * (it - t * n4));
+                if (live >> i & 1) val[i] = *(const float4 *)(x + (size_t)s_src[t] * ldx + 4 * (it - t * n4));
             }
         };
         fetch(blockIdx.x);
@@ -294,10 +315,11 @@ __global__ __launch_bounds__(KW_THREADS) void vx_kvq_write_kernel(vxh_kvq c, con
             const bool start = s_has[0] & 1;             // the page's first token starts it anew
             const float s_old = start ? 0.0f : held, sc = fmaxf(s_old, fit), inv = sc > 0.0f ? 1.0f / sc : 0.0f;
             const bool grown = sc > s_old && !start;
+            KW_HERE(live);
 #pragma unroll
             for (int i = 0; i < NI; i++) {
                 const int it = tid + i * KW_THREADS, t = token(it), d = 4 * (it - t * n4);
-                if (t < P && s_src[t] >= 0) {
+                if (live >> i & 1) {
                     const float a[4] = {val[i].x, val[i].y, val[i].z, val[i].w};
                     uint32_t code[4];
                     bool sure = finite && sc > 0.0f;
@@ -372,7 +394,10 @@ extern "C" int vxh_kvq_write(const vxh_kvq *c, const float *k, int ldk, const fl
     if (rc) return rc;
     // A prompt's pages begin every 32nd row or so: an odd piece length keeps the
     // workgroups that find one off one XCD (2048 rows, 32 heads of 128: 153 us
-    // with all on one, 37 spread; 512 pieces with 8192 workgroups 41).
+    // with all on one, 29 spread).  More pieces find the pages sooner, fewer
+    // leave each page to more workgroups: write and read-back of 2048 rows took
+    // 52 us with 256 pieces, 46 with 128, 46 with 64; of 1500 rows, 32 heads of
+    // 64, pages of 64: 51, 40, 39; of 2048 rows, 4 heads of 128: 16, 15, 19.
     const int chunk = R <= KW_PIECES ? 1 : (R + KW_PIECES - 1) / KW_PIECES | 1, gy = (R + chunk - 1) / chunk;
     int gx = 2 * c->n_kv_heads;
     if (gx > KW_WG / gy) gx = KW_WG / gy;
