@@ -26,15 +26,27 @@
 // and ending a tile cost.
 __device__ __forceinline__ int vx_kvq_weight(const vx_kvq_seq &s) { return vx_kvq_groups(s) + AK_BEGIN; }
 
-__device__ __forceinline__ void vx_dev_store2(float *p, float a, float b)
+// Partial results, that workgroups of other XCDs read: past this one's L2
+// (coherent over the device).  Offsets in floats: of a slot, and in it.
+typedef __amdgpu_buffer_rsrc_t vx_part;
+typedef unsigned int vx_u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int vx_u32x2 __attribute__((ext_vector_type(2)));
+#define AK_DEVICE 16             // the load's or store's scope
+__device__ __forceinline__ void vx_part_store(vx_part p, int slot, int at, vx_f32x4 v)
 {
-    __hip_atomic_store((uint64_t *)p, __builtin_bit_cast(uint64_t, make_float2(a, b)), __ATOMIC_RELAXED,
-                       __HIP_MEMORY_SCOPE_AGENT);
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(vx_u32x4, v), p, 4 * at, 4 * slot, AK_DEVICE);
 }
-__device__ __forceinline__ float2 vx_dev_load2(const float *p)
+__device__ __forceinline__ void vx_part_store2(vx_part p, int slot, int at, float a, float b)
 {
-    return __builtin_bit_cast(float2,
-                              __hip_atomic_load((const uint64_t *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(vx_u32x2, make_float2(a, b)), p, 4 * at, 4 * slot, AK_DEVICE);
+}
+__device__ __forceinline__ vx_f32x4 vx_part_load(vx_part p, int slot, int at)
+{
+    return __builtin_bit_cast(vx_f32x4, __builtin_amdgcn_raw_buffer_load_b128(p, 4 * at, 4 * slot, AK_DEVICE));
+}
+__device__ __forceinline__ float2 vx_part_load2(vx_part p, int slot, int at)
+{
+    return __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(p, 4 * at, 4 * slot, AK_DEVICE));
 }
 
 // Quotient of two counts; 64-bit division only where they need it.
@@ -192,7 +204,7 @@ __device__ __forceinline__ bool vx_arrive(unsigned *counter, int n, unsigned *s_
 // Parts i0..i1-1 of nv queries joined, in order, AK_JOIN at a time: their
 // loads wait for memory once.
 template <int HD, typename Slot, typename Out>
-__device__ __forceinline__ void vx_kvq_join(const float *part, Slot slot, int i0, int i1, int nv, Out put)
+__device__ __forceinline__ void vx_kvq_join(vx_part part, Slot slot, int i0, int i1, int nv, Out put)
 {
     constexpr int PS = HD + 4;
     for (int u = threadIdx.x; u < nv * (HD / 4); u += AK_THREADS) {
@@ -200,14 +212,14 @@ __device__ __forceinline__ void vx_kvq_join(const float *part, Slot slot, int i0
         float mx = -INFINITY, sum = 0.0f;
         vx_f32x4 o = vx_f32x4{};
         for (int p = i0; p < i1; p += AK_JOIN) {
-            float2 ml[AK_JOIN], v0[AK_JOIN], v1[AK_JOIN];
+            float2 ml[AK_JOIN];
+            vx_f32x4 v[AK_JOIN];
             float nm = mx;
 #pragma unroll
             for (int i = 0; i < AK_JOIN; i++) {
-                const float *pp = part + ((size_t)slot(min(p + i, i1 - 1)) * 16 + qq) * PS;
-                ml[i] = vx_dev_load2(pp + HD);
-                v0[i] = vx_dev_load2(pp + d);
-                v1[i] = vx_dev_load2(pp + d + 2);
+                const int at = slot(min(p + i, i1 - 1)) * (16 * PS);
+                ml[i] = vx_part_load2(part, at, qq * PS + HD);
+                v[i] = vx_part_load(part, at, qq * PS + d);
             }
 #pragma unroll
             for (int i = 0; i < AK_JOIN; i++) {
@@ -221,7 +233,7 @@ __device__ __forceinline__ void vx_kvq_join(const float *part, Slot slot, int i0
             for (int i = 0; i < AK_JOIN; i++) {
                 const float f = __builtin_amdgcn_exp2f(ml[i].x - ref);
                 sum = fmaf(ml[i].y, f, sum);
-                if (p + i < i1) o += vx_f32x4{v0[i].x, v0[i].y, v1[i].x, v1[i].y} * f;
+                if (p + i < i1) o += v[i] * f;
             }
             mx = nm;
         }
@@ -241,7 +253,7 @@ template <int TYPE, int HD>
 __global__ __launch_bounds__(AK_THREADS, 2) void vx_attention_kvq_kernel(
     vx_kvq_call c, const float *__restrict__ q, const int *__restrict__ table, const uint8_t *__restrict__ kc,
     const uint8_t *__restrict__ vc, const float *__restrict__ ks, const float *__restrict__ vs, float *__restrict__ out,
-    float *__restrict__ part, unsigned *__restrict__ counter)
+    float *__restrict__ parts, unsigned *__restrict__ counter)
 {
     constexpr int NJ = HD / 32, ND = HD / 16, PS = HD + 4;
     // the queries' operands, [tile][hi, lo][32 dims][lane]; after the last group
@@ -253,6 +265,7 @@ __global__ __launch_bounds__(AK_THREADS, 2) void vx_attention_kvq_kernel(
     __shared__ vx_kvq_list list;
     __shared__ unsigned s_last;
     const vx_kvq_batch &a = c.a;
+    const vx_part part = __builtin_amdgcn_make_buffer_rsrc((void *)parts, (short)0, 2 * AK_WG * 16 * PS * 4, 0x00020000);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, g4 = lane >> 4;
 
@@ -437,7 +450,7 @@ __global__ __launch_bounds__(AK_THREADS, 2) void vx_attention_kvq_kernel(
         __syncthreads();
         const bool whole = g_begin == 0 && g_end == groups;
         // a piece holds at most one tile begun before it and one that goes on behind it
-        float *mine_p = part + (size_t)(2 * blockIdx.x + (g_begin == 0)) * 16 * PS;
+        const int mine = (2 * (int)blockIdx.x + (g_begin == 0)) * (16 * PS);
         const int nv = min(16, s.nq - q0);
         for (int u = tid; u < nv * (HD / 4); u += AK_THREADS) {
             const int qq = u / (HD / 4), d = u % (HD / 4) * 4;
@@ -456,10 +469,8 @@ __global__ __launch_bounds__(AK_THREADS, 2) void vx_attention_kvq_kernel(
             if (whole)
                 finish(q0 + qq, d, o, sum);
             else {
-                float *pp = mine_p + (size_t)qq * PS;
-#pragma unroll
-                for (int e = 0; e < 4; e += 2) vx_dev_store2(pp + d + e, o[e], o[e + 1]);
-                if (d == 0) vx_dev_store2(pp + HD, mx, sum);
+                vx_part_store(part, mine, qq * PS + d, o);
+                if (d == 0) vx_part_store2(part, mine, qq * PS + HD, mx, sum);
             }
         }
         if (!whole) {
@@ -482,10 +493,8 @@ __global__ __launch_bounds__(AK_THREADS, 2) void vx_attention_kvq_kernel(
             if (last && n_blk > 1) {
                 if (c1 - c0 > 1)
                     vx_kvq_join<HD>(part, slot0, c0, c1, nv, [&](int qq, int d, vx_f32x4 o, float mx, float sum) {
-                        float *pp = part + ((size_t)slot1(blk) * 16 + qq) * PS;
-                        vx_dev_store2(pp + d, o[0], o[1]);
-                        vx_dev_store2(pp + d + 2, o[2], o[3]);
-                        if (d == 0) vx_dev_store2(pp + HD, mx, sum);
+                        vx_part_store(part, slot1(blk) * (16 * PS), qq * PS + d, o);
+                        if (d == 0) vx_part_store2(part, slot1(blk) * (16 * PS), qq * PS + HD, mx, sum);
                     });
                 last = vx_arrive(counter + AK_WG + p0, n_blk, &s_last);
             }
