@@ -13,13 +13,13 @@
 
 #define AK_WAVES 4
 #define AK_THREADS (64 * AK_WAVES)
-#define AK_WG 512                // pieces: two workgroups per CU
-#define AK_BEGIN 8               // what beginning and ending a tile costs, in 32-token groups
+#define AK_WG 512                // pieces: two workgroups per CU (640 and 768 pieces: the same or slower)
+#define AK_BEGIN 8               // what beginning and ending a tile costs, in 32-token groups (12: the same)
 #define AK_SMALL 8               // tiles of up to this many groups take a wavefront each
 #define AK_SNAP 12               // most groups a piece's end moves to a tile's
-#define AK_FEW 64                // queries per kv head up to which a request is this kernel's
+#define AK_FEW 64                // queries per kv head up to which a request is this kernel's (a tile of the other)
 #define AK_P 16384.0f            // what a probability is times in the matrix products
-#define AK_JOIN 8                // parts whose loads are in flight together
+#define AK_JOIN 8                // parts whose loads are in flight together (12, 16: one long request 62-64 us, not 60)
 #define AK_BLOCK 16              // parts one workgroup joins
 
 // Items of a tile: its groups, behind AK_BEGIN that stand for what beginning
@@ -248,6 +248,12 @@ __device__ __forceinline__ void vx_kvq_join(vx_part part, Slot slot, int i0, int
 // lane with tokens 4g..4g+3, 16+4g.. of query n, which is the operand P V
 // wants: no exchange between lanes but the maximum's.  The four wavefronts take
 // every fourth group and join in LDS; short tiles take a wavefront each.
+// Measured (28/4 heads of 128 unless said, kernel times): two requests of 128K
+// tokens 52 us for 269 MB (5.1 TB/s), 64 requests of up to 8K 50 us for 261 MB,
+// 16 requests of 9 rows at up to 2K with 32/32 heads 37 us for 150 MB: the
+// cache's bytes, and 2-3 us a tile begun and ended.  One request: 9 rows over
+// 8K 19 us, one row over 2K (32/4 heads of 64) 9 us: the chain of list, first
+// loads, groups, partial results, arrival and join.
 // ---------------------------------------------------------------------------
 template <int TYPE, int HD>
 __global__ __launch_bounds__(AK_THREADS, 2) void vx_attention_kvq_kernel(
