@@ -206,8 +206,9 @@ extern "C" int vxh_page_tables(const int *len, const int *add, int n_seqs, int p
 // Bound by HBM for a prompt: 2048 rows, 32 heads of 128, 29 us for 84 MB (2.9
 // TB/s; 65 pages x 16 workgroups, 4 parts each in turn, are four workgroups a
 // CU, and twice as many, each with its pass over the slots, are no faster), and
-// by latency below it: 5.0 us for one row of 4 heads, 7.9 for 64 rows on 64
-// pages (the slots, the rows, the old codes).
+// by latency below it: 4.8 us for one row of 4 heads, 8.0 for 64 rows on 64
+// pages (the slots, the rows, the old codes; the old codes asked for with the
+// rows, or the slots with the first rows': the same).
 // ---------------------------------------------------------------------------
 #define KW_THREADS 256
 #define KW_PIECES 128            // of the rows
@@ -430,8 +431,8 @@ extern "C" int vxh_kvq_write(const vxh_kvq *c, const float *k, int ldk, const fl
 // Read-back.  A workgroup takes 32 rows of one kv head's K or V.  Rows that are
 // 32 tokens of a page in order (a request read from its start) come as whole
 // lanes of the cache through LDS; any others code by code.
-// Bound by HBM: 2048 rows, 32 heads of 128, 15.2 us for 84 MB, 5.5 TB/s (36 us
-// when every value fetched its own byte); 64 single rows 7.4 us, latency.
+// Bound by HBM: 2048 rows, 32 heads of 128, 14.7 us for 84 MB, 5.7 TB/s (36 us
+// when every value fetched its own byte); 64 single rows 6.0 us, latency.
 // ---------------------------------------------------------------------------
 template <int TYPE>
 __global__ __launch_bounds__(256) void vx_kvq_read_kernel(vxh_kvq c, const int *__restrict__ slot, int R,
@@ -467,19 +468,41 @@ __global__ __launch_bounds__(256) void vx_kvq_read_kernel(vxh_kvq c, const int *
             *(float4 *)(x + (size_t)(r0 + i / n4) * ldx + 4 * (i % n4)) = *(const float4 *)&s_row[i / n4][4 * (i % n4)];
         return;
     }
-    for (int i = tid; i < 32 * n4; i += 256) {
-        const int r = r0 + i / n4, d = 4 * (i % n4), sl = r < R ? slot[r] : -1;
-        if (sl < 0 || (sl >> shift) >= c.n_pages) continue;
-        const int t = sl & ((1 << shift) - 1);
-        const size_t hp = (size_t)(sl >> shift) * c.n_kv_heads + head;
-        const uint8_t *p = codes + (hp << shift) * hd;
-        const float sc = scales[hp];
-        float f[4];
+    // (head_dim / 32 items a thread: the loads of all of them go out together)
+    int sl[4];
+    float sc[4];
+    uint32_t code[4][4];
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-            f[e] = vx_kvq_value<TYPE>(p[is_v ? vx_kvq_v_byte(t, d + e, hd) : vx_kvq_k_byte(t, d + e, hd)]) * sc;
-        *(float4 *)(x + (size_t)r * ldx + d) = make_float4(f[0], f[1], f[2], f[3]);
+    for (int j = 0; j < 4; j++) {
+        const int i = tid + j * 256, r = r0 + i / n4;
+        sl[j] = i < 32 * n4 && r < R ? slot[r] : -1;
+        if (sl[j] >= 0 && (sl[j] >> shift) >= c.n_pages) sl[j] = -1;
     }
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (sl[j] >= 0) {
+            const int d = 4 * ((tid + j * 256) % n4), t = sl[j] & ((1 << shift) - 1);
+            const size_t hp = (size_t)(sl[j] >> shift) * c.n_kv_heads + head;
+            const uint8_t *p = codes + (hp << shift) * hd;
+            sc[j] = scales[hp];
+            if (is_v) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) code[j][e] = p[vx_kvq_v_byte(t, d + e, hd)];
+            } else {
+                const uint32_t w = *(const uint32_t *)(p + vx_kvq_k_byte(t, d, hd));
+#pragma unroll
+                for (int e = 0; e < 4; e++) code[j][e] = w >> (8 * e) & 0xFFu;
+            }
+        }
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (sl[j] >= 0) {
+            const int i = tid + j * 256;
+            float f[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) f[e] = vx_kvq_value<TYPE>(code[j][e]) * sc[j];
+            *(float4 *)(x + (size_t)(r0 + i / n4) * ldx + 4 * (i % n4)) = make_float4(f[0], f[1], f[2], f[3]);
+        }
 }
 
 extern "C" int vxh_kvq_read(const vxh_kvq *c, const int *slot, int R, float *k, int ldk, float *v, int ldv,
