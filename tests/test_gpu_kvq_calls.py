@@ -236,3 +236,34 @@ def test_values_at_the_ends_of_fp32(P, rows, H, KV, size):
         check_attend(P, dc, oc, q, row0, [n], table, H, 0)
         check_attend(P, dc, oc, q, row0, [n], table, H, 0, max_seq_rows=1)
         dc.free()
+
+
+@pytest.mark.parametrize("kind", [Q.INT8, Q.E4M3])
+def test_most_rows_of_a_call(P, kind):
+    """The largest max_rows with a few rows in it, and with all but a few of them
+    one prompt's."""
+    page, hd, R = 32, 32, 1 << 18
+    rng = np.random.default_rng(77)
+    for adds in ([2, 1, 70], [1, R - 9, 3]):
+        lens = [300, max(adds[1], 40), 90]
+        print(f"attention: type {kind}, rows {adds} of {R}", flush=True)
+        pool, table, row0 = ragged(rng, lens, adds, page)
+        dc, oc = filled(P, kind, page, pool, 1, hd, rng)
+        q = rng.normal(0, 1, (row0[-1], hd)).astype(np.float32)
+        got = Q.run_attend(P, dc, q, row0, lens, table, 1, 100, max_rows=R, max_seq_rows=R)
+        assert np.all(got[row0[-1]:] == -3.0)
+        # 64 bits for the requests at both ends and for rows here and there between
+        pick = [0, 2] if adds[1] > 1000 else [0, 1, 2]
+        for b in pick:
+            rows = slice(row0[b], row0[b + 1])
+            want, tol = Q.attend(q[rows], oc, np.array([0, adds[b]]), lens[b:b + 1], table[b:b + 1], 1, 100,
+                                 np.zeros((adds[b], hd)))
+            assert np.all(np.abs(got[rows] - want).max(axis=1) <= tol)
+        if adds[1] > 1000:
+            for i in (0, 1, 63, 99, 100, 4097, adds[1] // 2, adds[1] - 1):
+                one = row0[1] + i
+                # row i of a prompt that began at position 0 reads as one row of i + 1 tokens
+                want, tol = Q.attend(q[one:one + 1], oc, np.array([0, 1]), [i + 1 + lens[1] - adds[1]], table[1:2], 1, 100,
+                                     np.zeros((1, hd)))
+                assert np.abs(got[one] - want[0]).max() <= tol[0], i
+        dc.free()

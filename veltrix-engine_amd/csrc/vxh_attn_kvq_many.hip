@@ -305,22 +305,28 @@ static int64_t vx_kvq_many_units(const vx_kvq_batch &a)
     return ((int64_t)a.max_rows * a.G + AM_QT - 1) / AM_QT * a.n_kv;
 }
 
+// Workgroups: a tile more per request with rows, for its last, partly filled one.
+static int64_t vx_kvq_many_grid(const vx_kvq_batch &a)
+{
+    const int with_rows = a.B < a.max_rows ? a.B : a.max_rows;
+    return vx_kvq_many_units(a) + (a.B > 1 ? (int64_t)with_rows * a.n_kv : 0);
+}
+
 // From 192 tiles on this kernel fills the card and beats the other one (200 tiles
 // of 1600 rows over 1900, 8/2 heads of 96: 36 us against 47; 192 of 768 rows,
 // 16/16 of 128: 23 against 30; 192 of 130 rows over 4130, 64/64 of 64: 52 against
 // 55); below, the other spreads the tiles' lengths too (128 tiles of 70 rows over
 // 3070, 64/64 of 64: 31 against 40; 96 of 192 over 2192, 32/32 of 128: 39
-// against 45).
+// against 45).  A launch holds less than 2^32 threads: 2^22 tiles.
 bool vx_kvq_many_wanted(const vx_kvq_batch &a, int max_seq_rows)
 {
-    return (int64_t)max_seq_rows * a.G > AM_QT && vx_kvq_many_units(a) >= 192;
+    return (int64_t)max_seq_rows * a.G > AM_QT && vx_kvq_many_units(a) >= 192 && vx_kvq_many_grid(a) <= 1 << 22;
 }
 
 int vx_kvq_many(const vx_kvq_call &c, int type, int head_dim, hipStream_t s)
 {
     const int64_t units = vx_kvq_many_units(c.a);
-    // a tile more per request for its last, partly filled one
-    const unsigned grid = (unsigned)(units + (c.a.B > 1 ? (int64_t)c.a.B * c.a.n_kv : 0));
+    const unsigned grid = (unsigned)vx_kvq_many_grid(c.a);
 #define VX_CALL(T, HD)                                                                                                \
     if (units < 384) vx_attention_kvq_many_kernel<T, HD, 4><<<grid, 1024, 0, s>>>(c);                                 \
     else vx_attention_kvq_many_kernel<T, HD, 2><<<grid, 512, 0, s>>>(c);
