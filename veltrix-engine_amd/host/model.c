@@ -361,8 +361,8 @@ static vx_error kv_tables(vx_model *m, int n_ctx)
     return VX_OK;
 }
 
-/* ints of a forward's step: len, add, len_out, row0[2], counts[4] */
-enum { KVQ_LEN = 0, KVQ_ADD = 1, KVQ_OUT = 2, KVQ_ROW0 = 3, KVQ_COUNTS = 5, KVQ_STEP_INTS = 9 };
+/* ints of a forward's step: len_out, row0[2], counts[4] */
+enum { KVQ_OUT = 0, KVQ_ROW0 = 1, KVQ_COUNTS = 3, KVQ_STEP_INTS = 7 };
 
 static vx_error kvq_alloc(vx_model *m, int n_ctx)
 {
@@ -371,14 +371,14 @@ static vx_error kvq_alloc(vx_model *m, int n_ctx)
     d->kvq_pages = (n_ctx + d->kvq_page - 1) / d->kvq_page;
     const size_t n_slots = (size_t)d->kvq_pages * d->kvq_page;
     d->kvq = (vxh_kvq *)calloc((size_t)L, sizeof(vxh_kvq));
-    int *ids = (int *)malloc(sizeof(int) * n_slots);
+    int *ids = (int *)malloc(sizeof(int) * (n_slots + 1));
     if (!d->kvq || !ids) { free(ids); return VX_ERR_MEMORY; }
-    for (size_t i = 0; i < n_slots; i++) ids[i] = (int)i;
+    for (size_t i = 0; i <= n_slots; i++) ids[i] = (int)i;
     int rc = VXH_OK;
     for (int l = 0; l < L && !rc; l++)
         rc = vxh_kvq_alloc(&d->kvq[l], d->kvq_type, d->kvq_page, d->kvq_pages, d->n_kv, d->hd);
-    if (!rc) rc = vxh_malloc((void **)&d->kvq_ids, sizeof(int) * n_slots);
-    if (!rc) rc = vxh_upload(d->kvq_ids, ids, sizeof(int) * n_slots, d->stream);
+    if (!rc) rc = vxh_malloc((void **)&d->kvq_ids, sizeof(int) * (n_slots + 1));
+    if (!rc) rc = vxh_upload(d->kvq_ids, ids, sizeof(int) * (n_slots + 1), d->stream);
     if (!rc) rc = vxh_malloc((void **)&d->kvq_table, sizeof(int) * (size_t)d->kvq_pages);
     if (!rc) rc = vxh_upload(d->kvq_table, ids, sizeof(int) * (size_t)d->kvq_pages, d->stream);
     free(ids);
@@ -967,13 +967,6 @@ static vx_error pgemm(vx_dev *d, const vxh_qmat *W, const vxh_pro *p, int M, dou
 }
 
 /* ---- the paged 8-bit cache ----------------------------------------------------- */
-static int fill_int(int *dst, int value, vxh_stream s)
-{
-    float f;                           /* the same 32 bits */
-    memcpy(&f, &value, sizeof f);
-    return vxh_fill_f32((float *)dst, f, 1, s);
-}
-
 /* The pages, slots and lengths of a forward of M rows at n_past.., for all of
  * its layers.  One row may stand past the context: it takes the last position,
  * as the reference's clamp does (src/model.c:279-286). */
@@ -989,9 +982,8 @@ static vx_error kvq_begin(vx_dev *d, int M, int n_past)
     }
     const int have = (n_past + d->kvq_page - 1) / d->kvq_page;
     int *st = d->kvq_step;
-    TRY(fill_int(st + KVQ_LEN, n_past, d->stream));
-    TRY(fill_int(st + KVQ_ADD, M, d->stream));
-    TRY(vxh_page_tables(st + KVQ_LEN, st + KVQ_ADD, 1, d->kvq_page, d->kvq_ids + have, d->kvq_pages - have,
+    /* the list of whole numbers holds the length and the rows, too */
+    TRY(vxh_page_tables(d->kvq_ids + n_past, d->kvq_ids + M, 1, d->kvq_page, d->kvq_ids + have, d->kvq_pages - have,
                         d->kvq_table, d->kvq_pages, st + KVQ_OUT, st + KVQ_ROW0, d->kvq_pos, d->kvq_slot, M,
                         st + KVQ_COUNTS, d->stream));
     return VX_OK;

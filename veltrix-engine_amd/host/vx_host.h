@@ -127,7 +127,7 @@ typedef struct vx_dev {
     int kvq_type, kvq_page;            /* 0: the cache of opt                     */
     vxh_kvq *kvq;                      /* [n_layers], allocated with the cache    */
     int kvq_pages;
-    int *kvq_ids;                      /* 0, 1, ..: the pages in order, and every slot */
+    int *kvq_ids;                      /* 0, 1, .. to the number of slots: the pages in order, every slot, lengths */
     int *kvq_table;                    /* [kvq_pages]                             */
     int *kvq_step;                     /* KVQ_STEP_INTS: a forward's lengths      */
     int *kvq_pos, *kvq_slot;           /* [VX_PF_ROWS]                            */
