@@ -278,11 +278,16 @@ __global__ __launch_bounds__(AK_THREADS, 2) void vx_attention_kvq_kernel(
     int64_t n_tiles;
     const int64_t total = vx_kvq_scan(a, list, &n_tiles);
     if (total == 0) return;
-    // pieces of whole rounds of the wavefronts, and no less than a sixteenth of
-    // an average tile where that is little
+    // Pieces of whole rounds of the wavefronts.  Where there is too little work for
+    // all, 8 groups at least, or what one block of parts a tile takes if that is no
+    // more than 20: a long tile's chain of groups costs more than a second level of
+    // joins, a short one's less (one request of 9 rows over 8192, 28/4 heads of 128:
+    // 19 us in 14 parts a tile, 23 in 22; 3 rows over 13000, 2/2 heads: 16 in 15
+    // parts, 13 in 52).
     int64_t piece = vx_quot(total + gridDim.x - 1, gridDim.x);
-    const int64_t part16 = min(max(vx_quot(total + n_tiles * AK_BLOCK - 1, n_tiles * AK_BLOCK), (int64_t)8), (int64_t)24);
-    piece = vx_uniform((max(piece, part16) + AK_WAVES - 1) / AK_WAVES * AK_WAVES);
+    int64_t least = vx_quot(total + n_tiles * AK_BLOCK - 1, n_tiles * AK_BLOCK);
+    least = least > 20 ? 8 : max(least, (int64_t)8);
+    piece = vx_uniform((max(piece, least) + AK_WAVES - 1) / AK_WAVES * AK_WAVES);
     // a boundary this near a tile's end moves there: beginning a tile costs more
     const int snap = __builtin_amdgcn_readfirstlane((int)min(piece / 4, (int64_t)AK_SNAP));
     const int64_t start = (int64_t)blockIdx.x * piece;
