@@ -4,8 +4,6 @@
 
 #include "vxh_internal.h"
 
-#define KVQ_MAX_PAGE 128
-
 // Byte of (token, dim) inside one page and head of the keys: 32 tokens x 32
 // dims are 1 KiB, lane 16 g + n of which holds dims 8g..8g+7 of token n, then
 // of token n + 16 -- the A operands of two 16x16x32 MFMAs in 16 bytes.
